@@ -102,9 +102,9 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // Dot-product arithmetic of the decode kernels (round 5; decode.hip, decode_layer.hip, decode_attn.h -- every GEMV and score of both
 // decode paths goes through these two, which is what keeps them bit-identical to each other): a lane accumulates TWO partial sums, the
-// even and the odd elements of its k range, by packed FMA (v_pk_fma_f32: two fp32 FMAs per instruction at the issue cost of one --
-// tools/pk_probe.hip), chunks ascending, and folds them lo + hi before the wave reduction.  A decode step is bound by the instruction
-// count of its single-wave chains (4 multiplies + 4 adds per chunk became 2 instructions), not by bytes or flops.
+// even and the odd elements of its k range, by explicit FMAs (v_fma_f32: the build has no packed fp32 instructions; with v_pk_fma_f32 the
+// same code measured 98.8 us per note, without it 98.3), chunks ascending, and folds them lo + hi before the wave reduction.  A decode
+// step is bound by the latency of its single-wave chains between the hand-offs, not by bytes or flops.
 __device__ __forceinline__ void dec_dot4(f32x2& a, const f32x4 w, const f32x4 x) {
     a = __builtin_elementwise_fma(f32x2{w[0], w[1]}, f32x2{x[0], x[1]}, a);
     a = __builtin_elementwise_fma(f32x2{w[2], w[3]}, f32x2{x[2], x[3]}, a);
@@ -112,8 +112,8 @@ __device__ __forceinline__ void dec_dot4(f32x2& a, const f32x4 w, const f32x4 x)
 __device__ __forceinline__ float dec_fold(const f32x2 a) { return a[0] + a[1]; }
 
 // LayerNorm statistics of the decode kernels (round 5), by ONE wave over the vector in the dot-product layout (lane owns the chunks
-// k = 4 lane + 256 c .. + 3, c < C; K a multiple of 4, entries past K ignored): two-pass, every lane folds its own entries first (packed
-// adds / FMAs, chunks ascending), then ONE wave_sum per pass.  Every wave that needs the normalised vector computes the statistics itself:
+// k = 4 lane + 256 c .. + 3, c < C; K a multiple of 4, entries past K ignored): two-pass, every lane folds its own entries first (even and
+// odd entries apart, chunks ascending), then ONE wave_sum per pass.  Every wave that needs the normalised vector computes the statistics itself:
 // no barrier, no partial sums through LDS (the 256-thread form -- four wave partials per pass exchanged through LDS, three barriers --
 // cost 0.76 us per call on the critical path of a note, twice per layer pair; recomputing those four partials in every wave 0.64).
 template <int C>

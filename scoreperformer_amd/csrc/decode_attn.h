@@ -34,7 +34,7 @@ __device__ __forceinline__ void dec_attn_batch(f32x4 (&k4)[NU], f32x4 (&v4)[NU],
     for (int u = 0; u < NU; ++u) {
         const int j = jb0 + G * u;
         f32x2 s2 = f32x2{0.f, 0.f};
-        dec_dot4(s2, q4, k4[u]);                // common.h: packed FMA, two partial sums
+        dec_dot4(s2, q4, k4[u]);                // common.h: two partial sums
         float s = row16_sum(dec_fold(s2));      // the 16 lanes of a key: one DPP row
         s -= slope * (float)(t - j);
         sc[u] = j < j1 ? s : -INFINITY;
@@ -46,7 +46,7 @@ __device__ __forceinline__ void dec_attn_batch(f32x4 (&k4)[NU], f32x4 (&v4)[NU],
     for (int u = 0; u < NU; ++u) {
         const float p = jb0 + G * u < j1 ? __expf(sc[u] - mb) : 0.f;
         lb += p;
-        ab_lo = __builtin_elementwise_fma(f32x2{v4[u][0], v4[u][1]}, f32x2{p, p}, ab_lo);   // two v_pk_fma_f32 per key
+        ab_lo = __builtin_elementwise_fma(f32x2{v4[u][0], v4[u][1]}, f32x2{p, p}, ab_lo);
         ab_hi = __builtin_elementwise_fma(f32x2{v4[u][2], v4[u][3]}, f32x2{p, p}, ab_hi);
     }
     const f32x4 ab = f32x4{ab_lo[0], ab_lo[1], ab_hi[0], ab_hi[1]};

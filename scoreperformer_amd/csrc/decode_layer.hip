@@ -13,11 +13,11 @@
 //   * epoch = tick * 256 + 8 * layer + phase + 1 with `tick` a device counter that the last pair launch of a note advances: tags never
 //     repeat within a render (the host zeroes the granule buffers when a render starts), also when a session re-decodes a position.
 // Arithmetic, association order and rounding are those of the five kernels it replaces, through helpers both files share: one wave per
-// output row, lanes own k = 4 lane + 256 c, two partial sums per lane by packed FMA (common.h dec_dot4); LayerNorm statistics per wave
+// output row, lanes own k = 4 lane + 256 c, two partial sums per lane (common.h dec_dot4); LayerNorm statistics per wave
 // over that layout (common.h dec_ln_stats); the split-key batches of dec_attn2_kernel (decode_attn.h: 8 keys per lane group, 32 lane
 // groups, two-level group merge); the 16-record split merge of dec_fused_gemv_kernel's prologue: the residual stream leaves bit-identical.
 // A decode step is bound by the INSTRUCTION COUNT of these single-wave chains between the hand-offs (tools/pk_probe.hip: a wave issues
-// ~one VALU instruction per 5 clocks whatever its neighbour on the SIMD does; packed fp32 issues at full rate), not by bytes or flops.
+// ~one VALU instruction per 5 clocks whatever its neighbour on the SIMD does), not by bytes or flops.
 // Every poll loop is bounded: a workgroup that never sees its tags sets *err and stops polling (the launch completes with garbage and
 // the host raises), it never hangs the device.
 //
@@ -167,7 +167,7 @@ __device__ __forceinline__ void load_row(f32x4 (&r)[C], const float* w, int K, i
 }
 // R rows against the vector in LDS: the vector's chunks are read ONCE for all rows and every step is branch-free (a row-by-row loop with
 // an exec-masked branch per chunk cost ~190 ns per row: 3.1 us for the 16 products of a feed-forward wave).  Per row the arithmetic is
-// the one of dec_fused_gemv_kernel: chunks ascending through common.h dec_dot4 (two partial sums per lane by packed FMA), folded, then
+// the one of dec_fused_gemv_kernel: chunks ascending through common.h dec_dot4 (two partial sums per lane), folded, then
 // the DPP ladder of wave_sum.
 template <int C, int R>
 __device__ __forceinline__ void dot_rows_x(const f32x4 (&r)[R][C], const f32x4 (&xv)[C], int K, int lane, float (&out)[R]);

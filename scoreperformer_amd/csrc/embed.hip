@@ -696,6 +696,9 @@ extern "C" int spn_embed_bwd(int nkeys, const float* const* tables, float* const
         const int nv = round_nv((D + 255) / 256);
         const int stats_blocks = spn_tune_i(SPN_TUNE_EMBED_STATS_BLOCKS) > 0 ? spn_tune_i(SPN_TUNE_EMBED_STATS_BLOCKS) : 2048;   // tuning aid (2048: -5 % over 1024; 256 or 16384: slower)
         int rpb = cdiv(T, stats_blocks); rpb = ((rpb + 3) / 4) * 4;
+        // a few short sequences: one block, so that dgamma / dbeta take ONE atomic add per column and do not depend on the order of blocks
+        // (an element whose terms cancel is otherwise noise of 1 % of itself from run to run; at these sizes the pass is launch-bound)
+        if (T <= 128) rpb = 128;
         dim3 grid(cdiv(T, rpb));
 #define CASE(NV_) case NV_: hipLaunchKernelGGL((embed_bwd_stats_kernel<NV_>), grid, dim3(256), 0, stream, d, tokens, tok_bs, tok_ts, t_len, (const bf16_t*)dy, lddy, gamma, mean, rstd, s1, s2, dgamma, dbeta, T, rpb); break;
         switch (nv) { CASE(1) CASE(2) CASE(4) CASE(6) CASE(8) default: return SPN_ERR_ARG; }
