@@ -407,6 +407,34 @@ int spn_dec_attn_rows(const float* q, long q_ld, const float* kcache, const floa
                       long o_ld, int h, int kvh, float scale, spn_stream_t s);
 int spn_dec_glu_rows(const float* u, long u_ld, float* out, long out_ld, int n, int I, int act, int glu, spn_stream_t s);
 
+/* ---- paged key / value cache: serving a batch of requests whose lengths differ and grow (the batched form of the cached decode step,
+ *      wrappers.py:325-407 with attention.py:155-156, where the reference concatenates per-batch caches every step).
+ *      Pages of `page` rows (a power of two in [8, 4096]): k_pages / v_pages [num_pages, kvh, page, 64]; block_table [R, W] int32 page ids
+ *      (row stride bt_ld; -1: none); lens [R] int32; the free pages are the first *num_free entries of free_pages [num_pages], taken from the
+ *      end.  Slot of a row = page id * page + row of the page.  Lengths, ids, counts and slots are device data and checked on the device: no
+ *      value of theirs leads outside the buffers.
+ *      spn_paged_plan: fresh [R] new rows per request (<= width) -> pages into block_table entries [pages(len), pages(len + fresh)), slots
+ *      [R, width] int64 (-1 behind fresh), lens_out, num_free_out (may be lens / num_free).  A request is served whole or not at all: refused
+ *      (all slots -1, length kept) with a count outside [0, width], a negative length, more pages than W, or none left behind the requests
+ *      before it (pages asked for by refused ones count too).
+ *      spn_paged_release: pages of the requests with done[r] back on the stack (page 0 of the first one on top), entries -1, lens 0.
+ *      spn_paged_append: rows k / v [T, kvh, 64] through element strides (row, head), dtype codes of rows and pages may differ; a slot outside
+ *      the pool skips its row.  Slots of one call are distinct.
+ *      spn_paged_attn: one query row per request, o[r, h] = softmax_j(scale q.k_j - slopes[h] (lens[r] - 1 - j)) v_j over j < lens[r]; fp32
+ *      arithmetic; q / o through (request, head) strides, q, pages and o of one dtype; slopes null: no bias.  No visible row: zeros.  Rows on an
+ *      entry outside [0, num_pages) are skipped, lengths are cut to W pages.  workspace: spn_paged_attn_workspace_bytes(R, h, kvh, W, page)
+ *      bytes, 16-byte aligned, used until the call's work is done (calls that may run at the same time need one each). */
+int spn_paged_plan(const int* lens, const int* fresh, int* block_table, long bt_ld, const int* free_pages, const int* num_free, int* lens_out,
+                   int* num_free_out, long long* slots, int R, int W, int num_pages, int page, int width, spn_stream_t s);
+int spn_paged_release(const uint8_t* done, int* lens, int* block_table, long bt_ld, int* free_pages, int* num_free, int R, int W,
+                      int num_pages, int page, spn_stream_t s);
+int spn_paged_append(const void* k, const void* v, int row_dtype, long k_rs, long k_hs, long v_rs, long v_hs, void* k_pages, void* v_pages,
+                     int page_dtype, const long long* slots, long T, int kvh, int num_pages, int page, spn_stream_t s);
+size_t spn_paged_attn_workspace_bytes(int R, int h, int kvh, int W, int page);
+int spn_paged_attn(const void* q, long q_rs, long q_hs, const void* k_pages, const void* v_pages, int dtype, const int* block_table,
+                   long bt_ld, const int* lens, const float* slopes, void* o, long o_rs, long o_hs, int R, int h, int kvh, int W,
+                   int num_pages, int page, float scale, void* workspace, size_t workspace_bytes, spn_stream_t s);
+
 /* ---- device-side batch builder (scoreperformer/data/collators/score_performance.py:35-115,186-234; performance.py:18-92,100-115,
  *      213-247): raw ragged int32 tokens (samples concatenated, row offsets [b+1]) -> every tensor the MixedLM collator returns:
  *      padded int64 tokens, bool masks, lengths, bar/beat/onset ids (seg_flat = [3, sum_s] or null), deadpan flags, masked_perf, labels.

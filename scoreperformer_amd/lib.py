@@ -36,11 +36,25 @@ def load() -> ctypes.CDLL:
         _lib.spn_attn_band_elems.restype = ctypes.c_long
         _lib.spn_gemm_workspace_bytes.restype = ctypes.c_size_t
         _lib.spn_tuning_name.restype = ctypes.c_char_p
+        for name, types in _SIGNATURES.items():
+            getattr(_lib, name).argtypes = types
+        _lib.spn_paged_attn_workspace_bytes.restype = ctypes.c_size_t
         if _lib.spn_abi_version() != ABI_VERSION:
             raise SpnError(f"{LIB_PATH} has ABI version {_lib.spn_abi_version()}, this package needs {ABI_VERSION}: rebuild it")
         _apply_env_tuning(_lib)
     return _lib
 
+
+# Argument types of entry points whose callers pass plain Python numbers and addresses (one conversion in C instead of a ctypes object per
+# argument: the calls of a decode step are bound by the host)
+_P, _I, _L, _F, _Z = c_void_p, c_int, c_long, c_float, ctypes.c_size_t
+_SIGNATURES = {
+    "spn_paged_plan": [_P] * 3 + [_L] + [_P] * 5 + [_I] * 5 + [_P],
+    "spn_paged_release": [_P] * 3 + [_L] + [_P] * 2 + [_I] * 4 + [_P],
+    "spn_paged_append": [_P] * 2 + [_I] + [_L] * 4 + [_P] * 2 + [_I, _P, _L] + [_I] * 3 + [_P],
+    "spn_paged_attn": [_P, _L, _L, _P, _P, _I, _P, _L, _P, _P, _P, _L, _L] + [_I] * 6 + [_F, _P, _Z, _P],
+    "spn_paged_attn_workspace_bytes": [_I] * 5,
+}
 
 ABI_VERSION = 10
 TUNING_EPOCH = 0

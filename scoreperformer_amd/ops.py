@@ -1410,3 +1410,177 @@ def collate_pad_tokens(flat, off, *, b, K, L, pad_id=0):
     lens = torch.empty(b, device=dev, dtype=torch.int64)
     call("spn_collate_pad_tokens", ptr(flat), ptr(off), c_int(b), c_int(K), c_int(L), c_int(pad_id), ptr(out), ptr(mask), ptr(lens), stream_ptr())
     return out, mask, lens
+
+
+# ---------------------------------------------------------------------------------------------------------
+# paged key / value cache (serving a batch of requests whose lengths differ and grow)
+# ---------------------------------------------------------------------------------------------------------
+
+PAGED_HEAD = 64   # head width of the attention kernels
+
+
+def _paged_check(name: str, ok: bool, what: str) -> None:
+    if not ok:
+        raise SpnError(f"{name}: {what}")
+
+
+def _paged_ints(name: str, arg: str, t: torch.Tensor, shape: Tuple[int, ...]) -> None:
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise SpnError(f"{name}: {arg} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+def _paged_size(name: str, page: int) -> None:
+    if page < 8 or page > 4096 or page & (page - 1):
+        raise SpnError(f"{name}: the page size must be a power of two in [8, 4096], got {page}")
+
+
+def _paged_table(name: str, t: torch.Tensor, page: int) -> Tuple[int, int, int]:
+    """[R, W] int32 with unit inner stride (a column slice of a wider table is fine) -> (R, W, row stride)."""
+    if t.dtype != torch.int32 or t.ndim != 2 or t.shape[1] < 1 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise SpnError(f"{name}: block_table must be int32 [requests, pages] with unit inner stride")
+    _paged_size(name, page)
+    R, W = t.shape
+    if W * page >= 2 ** 31 or R * W >= 2 ** 31:
+        raise SpnError(f"{name}: rows per request and table entries stay under 2^31, got a table {[R, W]} of pages of {page}")
+    return R, W, max(W, t.stride(0))
+
+
+def _paged_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
+    """All tensors on one GPU; returns it (the caller makes it current: the launch goes to ITS current stream)."""
+    require_gpu(*tensors)
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise SpnError(f"{name}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _paged_call(dev: torch.device, fn: str, *args) -> None:
+    """One launch on the current stream of `dev`, whichever device is current."""
+    if dev.index == torch.cuda.current_device():
+        call(fn, *args, stream_ptr())
+    else:
+        with torch.cuda.device(dev):
+            call(fn, *args, stream_ptr())
+
+
+def paged_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, num_free: torch.Tensor, page_size: int,
+               width: int, *, lens_out: Optional[torch.Tensor] = None, num_free_out: Optional[torch.Tensor] = None):
+    """Room for new rows: pages off the free stack into the block table, and the slot of every new row, without a host read.
+
+    lens [R] rows held and new [R] rows to come, int32; block_table [R, W] int32, updated in place: entries [pages(lens), pages(lens + new)) of a
+    served request; free_pages [num_pages] int32: the first num_free ([1] int32) are free, taken from the end.  Returns (slots int64 [R, width]:
+    page * page_size + row of the page for rows i < new, -1 behind them; lens_out [R]; num_free_out [1]).  lens_out may be `lens` and num_free_out
+    may be `num_free` (in place); otherwise neither is changed.
+
+    A request is served whole or not at all: with a count outside [0, width], a negative length, more rows than W pages hold, or no pages left
+    behind the requests before it, it gets no page, all its slots are -1 and its length stays (compare lens_out with lens + new)."""
+    n = "paged_plan"
+    R, W, ld = _paged_table(n, block_table, page_size)
+    _paged_ints(n, "lens", lens, (R,))
+    _paged_ints(n, "new", new, (R,))
+    _paged_check(n, free_pages.ndim == 1 and free_pages.numel() > 0, "free_pages must be [num_pages]")
+    _paged_ints(n, "free_pages", free_pages, (free_pages.numel(),))
+    _paged_ints(n, "num_free", num_free, (1,))
+    if lens_out is not None:
+        _paged_ints(n, "lens_out", lens_out, (R,))
+    if num_free_out is not None:
+        _paged_ints(n, "num_free_out", num_free_out, (1,))
+    _paged_check(n, width >= 1 and R * width < 2 ** 31, "width must be at least 1, requests x width under 2^31")
+    dev = _paged_device(n, lens, new, block_table, free_pages, num_free, lens_out, num_free_out)
+    slots = torch.empty((R, width), device=dev, dtype=torch.int64)
+    lens_out = torch.empty_like(lens) if lens_out is None else lens_out
+    num_free_out = torch.empty_like(num_free) if num_free_out is None else num_free_out
+    if R == 0:
+        num_free_out.copy_(num_free)
+        return slots, lens_out, num_free_out
+    _paged_call(dev, "spn_paged_plan", lens.data_ptr(), new.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(),
+                num_free.data_ptr(), lens_out.data_ptr(), num_free_out.data_ptr(), slots.data_ptr(), R, W, free_pages.numel(), page_size, width)
+    return slots, lens_out, num_free_out
+
+
+def paged_release(done: torch.Tensor, lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, num_free: torch.Tensor,
+                  page_size: int) -> None:
+    """The pages of the requests with done [R] (bool) go back on the free stack; their table entries become -1, their lengths 0.  All in place.
+    Page 0 of the first ended request ends on top: a plan for the same requests and lengths takes the same pages again.  A page belongs to one
+    request; entries outside [0, num_pages) are skipped."""
+    n = "paged_release"
+    R, W, ld = _paged_table(n, block_table, page_size)
+    _paged_check(n, done.dtype in (torch.bool, torch.uint8) and done.shape == (R,) and done.is_contiguous(), f"done must be contiguous bool [{R}]")
+    _paged_ints(n, "lens", lens, (R,))
+    _paged_check(n, free_pages.ndim == 1 and free_pages.numel() > 0, "free_pages must be [num_pages]")
+    _paged_ints(n, "free_pages", free_pages, (free_pages.numel(),))
+    _paged_ints(n, "num_free", num_free, (1,))
+    dev = _paged_device(n, done, lens, block_table, free_pages, num_free)
+    if R == 0:
+        return
+    _paged_call(dev, "spn_paged_release", done.data_ptr(), lens.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(),
+                num_free.data_ptr(), R, W, free_pages.numel(), page_size)
+
+
+def _paged_pools(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> Tuple[int, int, int]:
+    """[num_pages, kv_heads, page, 64], both alike -> (num_pages, kv_heads, page)."""
+    if k_pages.ndim != 4 or k_pages.shape[3] != PAGED_HEAD or 0 in k_pages.shape or not k_pages.is_contiguous():
+        raise SpnError(f"{name}: k_pages must be contiguous [num_pages, kv_heads, page, {PAGED_HEAD}], got {list(k_pages.shape)}")
+    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or not v_pages.is_contiguous():
+        raise SpnError(f"{name}: v_pages must be like k_pages")
+    return k_pages.shape[:3]
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor) -> None:
+    """Rows k, v [T, kv_heads, 64] (bf16 or fp32, unit inner stride: column slices of a fused projection buffer are read in place) into the slots
+    (int64, T of them, any shape; outside [0, num_pages * page): the row is skipped) of k_pages / v_pages [num_pages, kv_heads, page, 64], bf16
+    (fp32 rows are rounded to nearest even) or fp32.  The slots of one call are distinct: which of two rows for one slot stays is not defined."""
+    n = "paged_append"
+    num_pages, kvh, page = _paged_pools(n, k_pages, v_pages)
+    _paged_size(n, page)
+    _paged_check(n, k_pages.data_ptr() != v_pages.data_ptr(), "k_pages and v_pages are the same memory")
+    T = slots.numel()
+    for arg, t in (("k", k), ("v", v)):
+        if t.shape != (T, kvh, PAGED_HEAD) or t.stride(2) != 1:
+            raise SpnError(f"{n}: {arg} must be [{T}, {kvh}, {PAGED_HEAD}] with unit inner stride, got {list(t.shape)}")
+    _paged_check(n, k.dtype == v.dtype, "k and v must have one dtype")
+    rd, pd = _dt(k), _dt(k_pages)
+    _paged_check(n, slots.dtype == torch.int64 and slots.is_contiguous(), "slots must be contiguous int64")
+    _paged_check(n, T * kvh < 2 ** 31, "rows x heads stay under 2^31")
+    dev = _paged_device(n, k, v, k_pages, v_pages, slots)
+    if T == 0:
+        return
+    _paged_call(dev, "spn_paged_append", k.data_ptr(), v.data_ptr(), rd, k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_pages.data_ptr(),
+                v_pages.data_ptr(), pd, slots.data_ptr(), T, kvh, num_pages, page)
+
+
+def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
+               scale: Optional[float] = None, slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of ONE new row per request over its cached rows j < lens[r], the new row's own (the last) among them:
+    o = softmax_j(scale q.k_j - slopes[h] (lens[r] - 1 - j)) v_j.
+
+    q [R, h, 64] (any strides with unit inner stride) and the pages [num_pages, kv_heads, page, 64] both bf16 or both fp32; kv_heads divides h (1:
+    multi-query); block_table [R, W] and lens [R] int32; slopes [h] fp32 (ALiBi) or None; scale defaults to 1 / 8.  Returns [R, h, 64] in q's dtype
+    (`out` if given).  Scores, softmax and sums in fp32.  A request of length 0 has zeros.  Rows on an entry outside [0, num_pages) are skipped as if
+    masked (positions count on), rows behind a length are never read into a result, and a length past the table's W pages is cut to them.
+    No gradient: the training form is `attn_fwd` / `attn_bwd`."""
+    n = "paged_attn"
+    num_pages, kvh, page = _paged_pools(n, k_pages, v_pages)
+    R, W, ld = _paged_table(n, block_table, page)
+    if q.ndim != 3 or q.shape[0] != R or q.shape[2] != PAGED_HEAD or q.stride(2) != 1 or q.dtype != k_pages.dtype:
+        raise SpnError(f"{n}: q must be {k_pages.dtype} [{R}, heads, {PAGED_HEAD}] with unit inner stride, got {q.dtype} {list(q.shape)}")
+    h, dt = q.shape[1], _dt(q)
+    _paged_check(n, h > 0 and h % kvh == 0, f"{h} heads on {kvh} key heads")
+    _paged_ints(n, "lens", lens, (R,))
+    if slopes is not None and (slopes.dtype != F32 or slopes.shape != (h,) or not slopes.is_contiguous()):
+        raise SpnError(f"{n}: slopes must be contiguous fp32 [{h}]")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or (h > 1 and out.stride(1) < PAGED_HEAD)
+                            or (R > 1 and out.stride(0) < (h - 1) * out.stride(1) + PAGED_HEAD)):
+        raise SpnError(f"{n}: out must be like q with unit inner stride and rows that do not overlap")
+    dev = _paged_device(n, q, k_pages, v_pages, block_table, lens, slopes, out)
+    if out is None:
+        out = torch.empty((R, h, PAGED_HEAD), device=dev, dtype=q.dtype)
+    if R == 0:
+        return out
+    ws_bytes = load().spn_paged_attn_workspace_bytes(R, h, kvh, W, page)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+    _paged_call(dev, "spn_paged_attn", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), dt, block_table.data_ptr(),
+                ld, lens.data_ptr(), None if slopes is None else slopes.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), R, h,
+                kvh, W, num_pages, page, PAGED_HEAD ** -0.5 if scale is None else float(scale), None if ws is None else ws.data_ptr(), ws_bytes)
+    return out
