@@ -422,7 +422,7 @@ int spn_dec_glu_rows(const float* u, long u_ld, float* out, long out_ld, int n, 
  *      the pool skips its row.  Slots of one call are distinct.
  *      spn_paged_attn: one query row per request, o[r, h] = softmax_j(scale q.k_j - slopes[h] (lens[r] - 1 - j)) v_j over j < lens[r]; fp32
  *      arithmetic; q / o through (request, head) strides, q, pages and o of one dtype; slopes null: no bias.  No visible row: zeros.  Rows on an
- *      entry outside [0, num_pages) are skipped, lengths are cut to W pages.  workspace: spn_paged_attn_workspace_bytes(R, h, kvh, W, page)
+ *      entry outside [0, num_pages) are skipped, lengths are cut to W pages.  workspace: spn_paged_attn_workspace_bytes(R, h, kvh, W, page, dtype)
  *      bytes, 16-byte aligned, used until the call's work is done (calls that may run at the same time need one each). */
 int spn_paged_plan(const int* lens, const int* fresh, int* block_table, long bt_ld, const int* free_pages, const int* num_free, int* lens_out,
                    int* num_free_out, long long* slots, int R, int W, int num_pages, int page, int width, spn_stream_t s);
@@ -430,7 +430,7 @@ int spn_paged_release(const uint8_t* done, int* lens, int* block_table, long bt_
                       int num_pages, int page, spn_stream_t s);
 int spn_paged_append(const void* k, const void* v, int row_dtype, long k_rs, long k_hs, long v_rs, long v_hs, void* k_pages, void* v_pages,
                      int page_dtype, const long long* slots, long T, int kvh, int num_pages, int page, spn_stream_t s);
-size_t spn_paged_attn_workspace_bytes(int R, int h, int kvh, int W, int page);
+size_t spn_paged_attn_workspace_bytes(int R, int h, int kvh, int W, int page, int dtype);
 int spn_paged_attn(const void* q, long q_rs, long q_hs, const void* k_pages, const void* v_pages, int dtype, const int* block_table,
                    long bt_ld, const int* lens, const float* slopes, void* o, long o_rs, long o_hs, int R, int h, int kvh, int W,
                    int num_pages, int page, float scale, void* workspace, size_t workspace_bytes, spn_stream_t s);

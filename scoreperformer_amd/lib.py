@@ -53,7 +53,7 @@ _SIGNATURES = {
     "spn_paged_release": [_P] * 3 + [_L] + [_P] * 2 + [_I] * 4 + [_P],
     "spn_paged_append": [_P] * 2 + [_I] + [_L] * 4 + [_P] * 2 + [_I, _P, _L] + [_I] * 3 + [_P],
     "spn_paged_attn": [_P, _L, _L, _P, _P, _I, _P, _L, _P, _P, _P, _L, _L] + [_I] * 6 + [_F, _P, _Z, _P],
-    "spn_paged_attn_workspace_bytes": [_I] * 5,
+    "spn_paged_attn_workspace_bytes": [_I] * 6,
 }
 
 ABI_VERSION = 10

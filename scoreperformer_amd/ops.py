@@ -1578,7 +1578,7 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
         out = torch.empty((R, h, PAGED_HEAD), device=dev, dtype=q.dtype)
     if R == 0:
         return out
-    ws_bytes = load().spn_paged_attn_workspace_bytes(R, h, kvh, W, page)
+    ws_bytes = load().spn_paged_attn_workspace_bytes(R, h, kvh, W, page, dt)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
     _paged_call(dev, "spn_paged_attn", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), dt, block_table.data_ptr(),
                 ld, lens.data_ptr(), None if slopes is None else slopes.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), R, h,
