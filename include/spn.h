@@ -425,9 +425,11 @@ int spn_dec_glu_rows(const float* u, long u_ld, float* out, long out_ld, int n, 
  *      entry outside [0, num_pages) are skipped, lengths are cut to W pages.  workspace: spn_paged_attn_workspace_bytes(R, h, kvh, W, page, dtype)
  *      bytes, 16-byte aligned, used until the call's work is done (calls that may run at the same time need one each). */
 int spn_paged_plan(const int* lens, const int* fresh, int* block_table, long bt_ld, const int* free_pages, const int* num_free, int* lens_out,
-                   int* num_free_out, long long* slots, int R, int W, int num_pages, int page, int width, spn_stream_t s);
+                   int* num_free_out, long long* slots, int R, int W, int num_pages, int page, int width,
+                   void* workspace, size_t workspace_bytes, spn_stream_t s);
+size_t spn_paged_plan_workspace_bytes(int R, int width); /* 0: none needed */
 int spn_paged_release(const uint8_t* done, int* lens, int* block_table, long bt_ld, int* free_pages, int* num_free, int R, int W,
-                      int num_pages, int page, spn_stream_t s);
+                      int num_pages, int page, int* workspace /* R + 1 */, spn_stream_t s);
 int spn_paged_append(const void* k, const void* v, int row_dtype, long k_rs, long k_hs, long v_rs, long v_hs, void* k_pages, void* v_pages,
                      int page_dtype, const long long* slots, long T, int kvh, int num_pages, int page, spn_stream_t s);
 size_t spn_paged_attn_workspace_bytes(int R, int h, int kvh, int W, int page, int dtype);

@@ -26,7 +26,6 @@ using namespace spn_paged;
 namespace {
 
 constexpr int TILE = 32;       // rows per tile
-constexpr int WAVES = 4;       // waves per workgroup
 constexpr int HEADS = 16;      // query heads per pass
 constexpr int LDO = 68;        // LDS row of a head's o: 64 + 4, so that 16 heads do not meet in one bank
 constexpr float LOG2E_F = 1.4426950408889634f;
@@ -112,22 +111,23 @@ struct Walk {
         return PageIds{trow[min(at + (i >> 2) * 8, n - 1) >> a.shift], trow[min(at + g * 8, n - 1) >> a.shift]};
     }
 
-    __device__ __forceinline__ void load(X& x, int t, const PageIds id) const {
-        const int mask = (1 << a.shift) - 1, at = max(t, 0) * TILE;
-        x.ok = page_ok(id.v, a.num_pages);
-        // an entry that is no page: page 0's rows, masked below
-        const T* k = kp + row_offset(page_ok(id.k, a.num_pages) ? id.k : 0, 0, (at + (i >> 2) * 8) & mask, a.kvh, a.shift);
-        const T* v = vp + row_offset(x.ok ? id.v : 0, 0, (at + g * 8) & mask, a.kvh, a.shift);
+    // an entry that is no page: page 0's rows, masked by `ok`
+    __device__ __forceinline__ void load_k(X& x, int t, const PageIds id) const {
+        const T* k = kp + row_offset(page_ok(id.k, a.num_pages) ? id.k : 0, 0, (t * TILE + (i >> 2) * 8) & ((1 << a.shift) - 1), a.kvh, a.shift);
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int s = 0; s < X::PER; ++s) x.k[tt][s] = *reinterpret_cast<const typename X::K*>(k + tt * 4 * HEAD + s * (HEAD / X::PER));
+    }
+    __device__ __forceinline__ void load_v(X& x, int t, const PageIds id) const {
+        x.ok = page_ok(id.v, a.num_pages);
+        const T* v = vp + row_offset(x.ok ? id.v : 0, 0, (t * TILE + g * 8) & ((1 << a.shift) - 1), a.kvh, a.shift);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x.v[e] = *reinterpret_cast<const typename X::V*>(v + e * HEAD);
     }
 
-    __device__ __forceinline__ void compute(X& x, int t) {
-        f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    __device__ __forceinline__ void scores(const X& x, f32x4 (&s)[2]) const {
+        s[0] = f32x4{0.f, 0.f, 0.f, 0.f}; s[1] = s[0];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
             if constexpr (sizeof(T) == 2) {
@@ -140,6 +140,9 @@ struct Walk {
                     for (int f = 0; f < 4; ++f) s[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[tt][e][f], qf[e][f], s[tt], 0, 0, 0);
             }
         }
+    }
+
+    __device__ __forceinline__ void weigh(X& x, const f32x4 (&s)[2], int t) {
         const int row0 = t * TILE + g * 8;
         const float base = slope2 * (float)(row0 - (n - 1));
         float p[8];
@@ -195,24 +198,28 @@ struct Walk {
         }
     }
 
-    // tiles t, t - WAVES, ... down to t0: two tile buffers, page ids one tile ahead of the rows
+    // Tiles t, t - STEP, ... down to t0.  One tile's registers: the next tile's K replaces this one's as soon as its products are done, V the
+    // same behind the second product, and the page ids come a tile earlier.  Loads return in order, so they are issued in the order of their
+    // use (K, ids, V) and every wait leaves the younger ones in flight.
+    template <int STEP>
     __device__ __forceinline__ void run(int t, int t0) {
         if (t < t0) return;
-        X x, y;
+        X x;
         PageIds id = pages(t);
-        load(x, t, id);
-        id = pages(t - WAVES);
+        load_k(x, t, id);
+        PageIds next = pages(t - STEP);
+        load_v(x, t, id);
         for (;;) {
-            PageIds next = pages(t - 2 * WAVES);
-            if (t - WAVES >= t0) load(y, t - WAVES, id);
-            compute(x, t);
-            if ((t -= WAVES) < t0) return;
+            f32x4 s[2];
+            scores(x, s);
+            const bool more = t - STEP >= t0;
             id = next;
-            next = pages(t - 2 * WAVES);
-            if (t - WAVES >= t0) load(x, t - WAVES, id);
-            compute(y, t);
-            if ((t -= WAVES) < t0) return;
-            id = next;
+            if (more) load_k(x, t - STEP, id);
+            next = pages(t - 2 * STEP);
+            weigh(x, s, t);
+            if (!more) return;
+            t -= STEP;
+            load_v(x, t, id);
         }
     }
 };
@@ -230,8 +237,8 @@ __device__ __forceinline__ void store4(T* to, const float (&v)[4]) {   // any al
 }
 
 // DIRECT: workgroup = one (request, key head, pass), no cut.  Otherwise the G-th part of the line of tiles.
-template <typename T, bool DIRECT>
-__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 3 : 2) void paged_attn_kernel(PagedAttnArgs a) {
+template <typename T, bool DIRECT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 4 : 3) void paged_attn_kernel(PagedAttnArgs a) {
     __shared__ float s_o[WAVES][HEADS][LDO], s_m[WAVES][HEADS], s_l[WAVES][HEADS];
     __shared__ long s_sum[WAVES], s_at[3];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), H = a.kvh * a.passes;
@@ -300,14 +307,14 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 ? 3 : 2) void paged_attn
         }
         const int kh = hp / a.passes, first = (hp - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
         wk.begin(r, n, kh, head0, heads);
-        wk.run(t1 - 1 - w, t0);
+        wk.template run<WAVES>(t1 - 1 - w, t0);
         const float l = quad_sum(wk.l);
         if (wk.g == 0) { s_m[w][wk.i] = wk.m; s_l[w][wk.i] = l; }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             *reinterpret_cast<f32x4*>(&s_o[w][wk.i][16 * wk.g + 4 * q]) = f32x4{wk.o[0][q], wk.o[1][q], wk.o[2][q], wk.o[3][q]};
         __syncthreads();
-        const int hd = tid >> 4, d = (tid & 15) * 4;
+        const int hd = tid >> 4, d = (tid & 15) * 4;   // the first 256 threads: 16 heads x 16 pieces of 4 dimensions
         if (hd < heads) {
             float M = -__builtin_inff(), L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -383,8 +390,21 @@ __global__ __launch_bounds__(256 * JOIN) void paged_join_kernel(PagedAttnArgs a)
     }
 }
 
-constexpr int MIN_TILES = 8;       // two tiles a wave
-constexpr int DIRECT_ROWS = 256;   // tables of at most this many rows: a workgroup per (request, key head)
+#ifndef PA_MIN_TILES
+#define PA_MIN_TILES 8
+#endif
+#ifndef PA_DIRECT_ROWS
+#define PA_DIRECT_ROWS 256
+#endif
+#ifndef PA_SPLIT_WAVES
+#define PA_SPLIT_WAVES 4
+#endif
+#ifndef PA_DIRECT_WAVES
+#define PA_DIRECT_WAVES 4
+#endif
+constexpr int MIN_TILES = PA_MIN_TILES;       // two tiles a wave
+constexpr int DIRECT_ROWS = PA_DIRECT_ROWS;   // tables of at most this many rows: a workgroup per (request, key head)
+constexpr int SPLIT_WAVES = PA_SPLIT_WAVES, DIRECT_WAVES = PA_DIRECT_WAVES;
 
 struct Split { long grid; bool direct; int passes, rows; };
 Split split_of(int R, int h, int kvh, int W, int shift, int esize) {
@@ -393,7 +413,7 @@ Split split_of(int R, int h, int kvh, int W, int shift, int esize) {
     s.passes = (group + HEADS - 1) / HEADS; s.rows = group < HEADS ? group : HEADS;
     const long H = (long)kvh * s.passes, cap = (long)W << shift, tiles = (cap + TILE - 1) / TILE;
     s.direct = cap <= DIRECT_ROWS;
-    const long most = 256 * (esize == 2 ? 3 : 2), units = (tiles * H + MIN_TILES - 1) / MIN_TILES * R;
+    const long most = 256 * (esize == 2 ? 4 : 3) * 4 / SPLIT_WAVES, units = (tiles * H + MIN_TILES - 1) / MIN_TILES * R;
     s.grid = s.direct ? R * H : units < most ? units : most;
     return s;
 }
@@ -404,6 +424,18 @@ int page_shift(int page) {
 }
 
 size_t scratch_of(const Split& s) { return s.direct ? 0 : (size_t)s.grid * (2 * (size_t)s.rows * (HEAD + 2) * sizeof(float) + sizeof(int4)); }
+
+template <typename T, bool DIRECT>
+int launch(const PagedAttnArgs& a, long grid, hipStream_t stream) {
+    constexpr int WAVES = DIRECT ? DIRECT_WAVES : SPLIT_WAVES;
+    hipLaunchKernelGGL((paged_attn_kernel<T, DIRECT, WAVES>), dim3((unsigned)grid), dim3(64 * WAVES), 0, stream, a);
+    SPN_LAUNCH_CHECK();
+    if (!DIRECT) {
+        hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)grid), dim3(256 * JOIN), 0, stream, a);
+        SPN_LAUNCH_CHECK();
+    }
+    return SPN_OK;
+}
 
 }  // namespace
 
@@ -432,19 +464,6 @@ extern "C" int spn_paged_attn(const void* q, long q_rs, long q_hs, const void* k
     if (!s.direct) {
         a.hdr = (int4*)workspace; a.part = (float*)(a.hdr + s.grid); a.ml = a.part + 2 * s.grid * s.rows * HEAD;
     }
-    const dim3 grid((unsigned)s.grid), block(64 * WAVES);
-    if (s.direct) {
-        if (dtype == 1) hipLaunchKernelGGL((paged_attn_kernel<bf16_t, true>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((paged_attn_kernel<float, true>), grid, block, 0, stream, a);
-    } else if (dtype == 1) {
-        hipLaunchKernelGGL((paged_attn_kernel<bf16_t, false>), grid, block, 0, stream, a);
-        SPN_LAUNCH_CHECK();
-        hipLaunchKernelGGL(paged_join_kernel<bf16_t>, grid, dim3(256 * JOIN), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((paged_attn_kernel<float, false>), grid, block, 0, stream, a);
-        SPN_LAUNCH_CHECK();
-        hipLaunchKernelGGL(paged_join_kernel<float>, grid, dim3(256 * JOIN), 0, stream, a);
-    }
-    SPN_LAUNCH_CHECK();
-    return SPN_OK;
+    if (dtype == 1) return s.direct ? launch<bf16_t, true>(a, s.grid, stream) : launch<bf16_t, false>(a, s.grid, stream);
+    return s.direct ? launch<float, true>(a, s.grid, stream) : launch<float, false>(a, s.grid, stream);
 }

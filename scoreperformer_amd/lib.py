@@ -38,7 +38,7 @@ def load() -> ctypes.CDLL:
         _lib.spn_tuning_name.restype = ctypes.c_char_p
         for name, types in _SIGNATURES.items():
             getattr(_lib, name).argtypes = types
-        _lib.spn_paged_attn_workspace_bytes.restype = ctypes.c_size_t
+        _lib.spn_paged_attn_workspace_bytes.restype = _lib.spn_paged_plan_workspace_bytes.restype = ctypes.c_size_t
         if _lib.spn_abi_version() != ABI_VERSION:
             raise SpnError(f"{LIB_PATH} has ABI version {_lib.spn_abi_version()}, this package needs {ABI_VERSION}: rebuild it")
         _apply_env_tuning(_lib)
@@ -49,8 +49,9 @@ def load() -> ctypes.CDLL:
 # argument: the calls of a decode step are bound by the host)
 _P, _I, _L, _F, _Z = c_void_p, c_int, c_long, c_float, ctypes.c_size_t
 _SIGNATURES = {
-    "spn_paged_plan": [_P] * 3 + [_L] + [_P] * 5 + [_I] * 5 + [_P],
-    "spn_paged_release": [_P] * 3 + [_L] + [_P] * 2 + [_I] * 4 + [_P],
+    "spn_paged_plan": [_P] * 3 + [_L] + [_P] * 5 + [_I] * 5 + [_P, _Z, _P],
+    "spn_paged_plan_workspace_bytes": [_I] * 2,
+    "spn_paged_release": [_P] * 3 + [_L] + [_P] * 2 + [_I] * 4 + [_P, _P],
     "spn_paged_append": [_P] * 2 + [_I] + [_L] * 4 + [_P] * 2 + [_I, _P, _L] + [_I] * 3 + [_P],
     "spn_paged_attn": [_P, _L, _L, _P, _P, _I, _P, _L, _P, _P, _P, _L, _L] + [_I] * 6 + [_F, _P, _Z, _P],
     "spn_paged_attn_workspace_bytes": [_I] * 6,
@@ -96,6 +97,11 @@ def ptr(t: Optional[torch.Tensor]):
 
 def stream_ptr() -> c_void_p:
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of GPU `index` as a number (what stream_ptr() wraps, without building a torch.cuda.Stream: 0.1 us instead of 2.9)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def call(name: str, *args) -> None:

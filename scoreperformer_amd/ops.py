@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import lib as _lib_mod
-from .lib import load,  call, ptr, stream_ptr, require_gpu, c_int, c_long, c_float, SpnError
+from .lib import load,  call, ptr, stream_ptr, raw_stream, require_gpu, c_int, c_long, c_float, SpnError
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -1446,22 +1446,22 @@ def _paged_table(name: str, t: torch.Tensor, page: int) -> Tuple[int, int, int]:
 
 
 def _paged_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
-    """All tensors on one GPU; returns it (the caller makes it current: the launch goes to ITS current stream)."""
-    require_gpu(*tensors)
-    dev = tensors[0].device
+    """All tensors on one GPU; returns it."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise SpnError(f"{name}: tensors on {dev} and {t.device}")
-    return dev
+        if t is not None and t.get_device() != index or index < 0:
+            require_gpu(*tensors)
+            raise SpnError(f"{name}: tensors on {tensors[0].device} and {t.device}")
+    return tensors[0].device
 
 
 def _paged_call(dev: torch.device, fn: str, *args) -> None:
-    """One launch on the current stream of `dev`, whichever device is current."""
+    """The call on the current stream of `dev`, whichever device is current."""
     if dev.index == torch.cuda.current_device():
-        call(fn, *args, stream_ptr())
+        call(fn, *args, raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            call(fn, *args, stream_ptr())
+            call(fn, *args, raw_stream(dev.index))
 
 
 def paged_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, num_free: torch.Tensor, page_size: int,
@@ -1494,8 +1494,11 @@ def paged_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor,
     if R == 0:
         num_free_out.copy_(num_free)
         return slots, lens_out, num_free_out
+    ws_bytes = load().spn_paged_plan_workspace_bytes(R, width)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
     _paged_call(dev, "spn_paged_plan", lens.data_ptr(), new.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(),
-                num_free.data_ptr(), lens_out.data_ptr(), num_free_out.data_ptr(), slots.data_ptr(), R, W, free_pages.numel(), page_size, width)
+                num_free.data_ptr(), lens_out.data_ptr(), num_free_out.data_ptr(), slots.data_ptr(), R, W, free_pages.numel(), page_size, width,
+                None if ws is None else ws.data_ptr(), ws_bytes)
     return slots, lens_out, num_free_out
 
 
@@ -1514,8 +1517,9 @@ def paged_release(done: torch.Tensor, lens: torch.Tensor, block_table: torch.Ten
     dev = _paged_device(n, done, lens, block_table, free_pages, num_free)
     if R == 0:
         return
+    ws = torch.empty(R + 1, device=dev, dtype=torch.int32)
     _paged_call(dev, "spn_paged_release", done.data_ptr(), lens.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(),
-                num_free.data_ptr(), R, W, free_pages.numel(), page_size)
+                num_free.data_ptr(), R, W, free_pages.numel(), page_size, ws.data_ptr())
 
 
 def _paged_pools(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> Tuple[int, int, int]:
@@ -1542,7 +1546,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     _paged_check(n, k.dtype == v.dtype, "k and v must have one dtype")
     rd, pd = _dt(k), _dt(k_pages)
     _paged_check(n, slots.dtype == torch.int64 and slots.is_contiguous(), "slots must be contiguous int64")
-    _paged_check(n, T * kvh < 2 ** 31, "rows x heads stay under 2^31")
+    _paged_check(n, T * kvh < 2 ** 28, "rows x heads stay under 2^28")
     dev = _paged_device(n, k, v, k_pages, v_pages, slots)
     if T == 0:
         return
