@@ -244,7 +244,7 @@ extern "C" int spn_paged_plan(const int* lens, const int* fresh, int* block_tabl
     const int shift = log2_page(page);
     SPN_REQUIRE(lens && fresh && block_table && free_pages && num_free && lens_out && num_free_out && slots, "spn_paged_plan: null buffer");
     SPN_REQUIRE(shift >= 0, "spn_paged_plan: the page size must be a power of two in [8, 4096]");
-    SPN_REQUIRE(R > 0 && W > 0 && num_pages > 0 && width > 0 && bt_ld >= W, "spn_paged_plan: bad sizes");
+    SPN_REQUIRE(R > 0 && R < (1 << 24) && W > 0 && num_pages > 0 && width > 0 && bt_ld >= W, "spn_paged_plan: bad sizes");
     SPN_REQUIRE((long)R * W < (1L << 31) && ((long)W << shift) < (1L << 31) && (long)R * width < (1L << 31), "spn_paged_plan: sizes pass 2^31");
     const size_t need = spn_paged_plan_workspace_bytes(R, width);
     SPN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
@@ -265,7 +265,7 @@ extern "C" int spn_paged_release(const uint8_t* done, int* lens, int* block_tabl
     const int shift = log2_page(page);
     SPN_REQUIRE(done && lens && block_table && free_pages && num_free && workspace, "spn_paged_release: null buffer");
     SPN_REQUIRE(shift >= 0, "spn_paged_release: the page size must be a power of two in [8, 4096]");
-    SPN_REQUIRE(R > 0 && W > 0 && num_pages > 0 && bt_ld >= W && (long)R * W < (1L << 31), "spn_paged_release: bad sizes");
+    SPN_REQUIRE(R > 0 && R < (1 << 24) && W > 0 && num_pages > 0 && bt_ld >= W && (long)R * W < (1L << 31), "spn_paged_release: bad sizes");
     const ReleaseArgs a{done, lens, block_table, bt_ld, free_pages, num_free, R, W, num_pages, shift, workspace};
     hipLaunchKernelGGL(release_count_kernel, dim3(cdiv(R, 4)), dim3(256), 0, stream, a);
     SPN_LAUNCH_CHECK();
@@ -280,7 +280,7 @@ extern "C" int spn_paged_append(const void* k, const void* v, int row_dtype, lon
     SPN_REQUIRE(k && v && k_pages && v_pages && slots, "spn_paged_append: null buffer");
     SPN_REQUIRE((row_dtype | page_dtype) >> 1 == 0, "spn_paged_append: dtype codes are 0 (fp32) and 1 (bf16)");
     SPN_REQUIRE(shift >= 0, "spn_paged_append: the page size must be a power of two in [8, 4096]");
-    SPN_REQUIRE(T > 0 && kvh > 0 && num_pages > 0 && T * kvh < (1L << 28), "spn_paged_append: bad sizes");
+    SPN_REQUIRE(T > 0 && kvh > 0 && num_pages > 0 && T * kvh < (1L << 26), "spn_paged_append: bad sizes");
     const AppendArgs a{k, v, k_rs, k_hs, v_rs, v_hs, k_pages, v_pages, slots, T, kvh, num_pages, shift};
     if (row_dtype == 0 && page_dtype == 0) append_launch<float, float>(a, stream);
     else if (row_dtype == 0) append_launch<float, bf16_t>(a, stream);

@@ -1419,14 +1419,17 @@ def collate_pad_tokens(flat, off, *, b, K, L, pad_id=0):
 PAGED_HEAD = 64   # head width of the attention kernels
 
 
+# A decode step is a handful of small launches, so these wrappers are what it costs (a launch is 2.7 us of host time): sizes are unpacked
+# once, every check is a comparison, and messages are built only when one fails.
+
 def _paged_check(name: str, ok: bool, what: str) -> None:
     if not ok:
         raise SpnError(f"{name}: {what}")
 
 
-def _paged_ints(name: str, arg: str, t: torch.Tensor, shape: Tuple[int, ...]) -> None:
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise SpnError(f"{name}: {arg} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+def _paged_ints(name: str, arg: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype is not torch.int32 or t.ndim != 1 or t.numel() != n or not t.is_contiguous():
+        raise SpnError(f"{name}: {arg} must be contiguous int32 [{n}], got {t.dtype} {list(t.shape)}")
 
 
 def _paged_size(name: str, page: int) -> None:
@@ -1436,13 +1439,28 @@ def _paged_size(name: str, page: int) -> None:
 
 def _paged_table(name: str, t: torch.Tensor, page: int) -> Tuple[int, int, int]:
     """[R, W] int32 with unit inner stride (a column slice of a wider table is fine) -> (R, W, row stride)."""
-    if t.dtype != torch.int32 or t.ndim != 2 or t.shape[1] < 1 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise SpnError(f"{name}: block_table must be int32 [requests, pages] with unit inner stride")
     _paged_size(name, page)
-    R, W = t.shape
-    if W * page >= 2 ** 31 or R * W >= 2 ** 31:
-        raise SpnError(f"{name}: rows per request and table entries stay under 2^31, got a table {[R, W]} of pages of {page}")
-    return R, W, max(W, t.stride(0))
+    if t.dtype is not torch.int32 or t.ndim != 2:
+        raise SpnError(f"{name}: block_table must be int32 [requests, pages], got {t.dtype} {list(t.shape)}")
+    (R, W), (ld, inner) = t.shape, t.stride()
+    if W < 1 or (inner != 1 and W > 1) or (R > 1 and ld < W):
+        raise SpnError(f"{name}: block_table must have pages and unit inner stride, got {[R, W]} with strides {[ld, inner]}")
+    if W * page >= 2 ** 31 or R * W >= 2 ** 31 or R >= 2 ** 24:
+        raise SpnError(f"{name}: rows per request and table entries stay under 2^31, requests under 2^24, got a table {[R, W]} of pages of {page}")
+    return R, W, ld if ld > W else W
+
+
+def _paged_pools(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> Tuple[int, int, int]:
+    """[num_pages, kv_heads, page, 64], both alike -> (num_pages, kv_heads, page)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[3] != PAGED_HEAD or k_pages.numel() == 0 or not k_pages.is_contiguous():
+        raise SpnError(f"{name}: k_pages must be contiguous [num_pages, kv_heads, page, {PAGED_HEAD}], got {list(shape)}")
+    if v_pages.shape != shape or v_pages.dtype is not k_pages.dtype or not v_pages.is_contiguous():
+        raise SpnError(f"{name}: v_pages must be like k_pages")
+    n, kvh, page, _ = shape
+    if kvh * page >= 2 ** 24:
+        raise SpnError(f"{name}: a page's key heads x rows stay under 2^24, got {kvh} x {page}")
+    return n, kvh, page
 
 
 def _paged_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
@@ -1457,11 +1475,12 @@ def _paged_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
 
 def _paged_call(dev: torch.device, fn: str, *args) -> None:
     """The call on the current stream of `dev`, whichever device is current."""
-    if dev.index == torch.cuda.current_device():
-        call(fn, *args, raw_stream(dev.index))
+    index = dev.index
+    if index == torch.cuda.current_device():
+        call(fn, *args, raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            call(fn, *args, raw_stream(dev.index))
+            call(fn, *args, raw_stream(index))
 
 
 def paged_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, num_free: torch.Tensor, page_size: int,
@@ -1477,15 +1496,14 @@ def paged_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor,
     behind the requests before it, it gets no page, all its slots are -1 and its length stays (compare lens_out with lens + new)."""
     n = "paged_plan"
     R, W, ld = _paged_table(n, block_table, page_size)
-    _paged_ints(n, "lens", lens, (R,))
-    _paged_ints(n, "new", new, (R,))
-    _paged_check(n, free_pages.ndim == 1 and free_pages.numel() > 0, "free_pages must be [num_pages]")
-    _paged_ints(n, "free_pages", free_pages, (free_pages.numel(),))
-    _paged_ints(n, "num_free", num_free, (1,))
+    _paged_ints(n, "lens", lens, R)
+    _paged_ints(n, "new", new, R)
+    _paged_ints(n, "free_pages", free_pages, free_pages.numel() or 1)
+    _paged_ints(n, "num_free", num_free, 1)
     if lens_out is not None:
-        _paged_ints(n, "lens_out", lens_out, (R,))
+        _paged_ints(n, "lens_out", lens_out, R)
     if num_free_out is not None:
-        _paged_ints(n, "num_free_out", num_free_out, (1,))
+        _paged_ints(n, "num_free_out", num_free_out, 1)
     _paged_check(n, width >= 1 and R * width < 2 ** 31, "width must be at least 1, requests x width under 2^31")
     dev = _paged_device(n, lens, new, block_table, free_pages, num_free, lens_out, num_free_out)
     slots = torch.empty((R, width), device=dev, dtype=torch.int64)
@@ -1494,7 +1512,7 @@ def paged_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor,
     if R == 0:
         num_free_out.copy_(num_free)
         return slots, lens_out, num_free_out
-    ws_bytes = load().spn_paged_plan_workspace_bytes(R, width)
+    ws_bytes = load().spn_paged_plan_workspace_bytes(R, width) if R * width > 1024 else 0   # (never for fewer slots)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
     _paged_call(dev, "spn_paged_plan", lens.data_ptr(), new.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(),
                 num_free.data_ptr(), lens_out.data_ptr(), num_free_out.data_ptr(), slots.data_ptr(), R, W, free_pages.numel(), page_size, width,
@@ -1510,25 +1528,15 @@ def paged_release(done: torch.Tensor, lens: torch.Tensor, block_table: torch.Ten
     n = "paged_release"
     R, W, ld = _paged_table(n, block_table, page_size)
     _paged_check(n, done.dtype in (torch.bool, torch.uint8) and done.shape == (R,) and done.is_contiguous(), f"done must be contiguous bool [{R}]")
-    _paged_ints(n, "lens", lens, (R,))
-    _paged_check(n, free_pages.ndim == 1 and free_pages.numel() > 0, "free_pages must be [num_pages]")
-    _paged_ints(n, "free_pages", free_pages, (free_pages.numel(),))
-    _paged_ints(n, "num_free", num_free, (1,))
+    _paged_ints(n, "lens", lens, R)
+    _paged_ints(n, "free_pages", free_pages, free_pages.numel() or 1)
+    _paged_ints(n, "num_free", num_free, 1)
     dev = _paged_device(n, done, lens, block_table, free_pages, num_free)
     if R == 0:
         return
     ws = torch.empty(R + 1, device=dev, dtype=torch.int32)
     _paged_call(dev, "spn_paged_release", done.data_ptr(), lens.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(),
                 num_free.data_ptr(), R, W, free_pages.numel(), page_size, ws.data_ptr())
-
-
-def _paged_pools(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> Tuple[int, int, int]:
-    """[num_pages, kv_heads, page, 64], both alike -> (num_pages, kv_heads, page)."""
-    if k_pages.ndim != 4 or k_pages.shape[3] != PAGED_HEAD or 0 in k_pages.shape or not k_pages.is_contiguous():
-        raise SpnError(f"{name}: k_pages must be contiguous [num_pages, kv_heads, page, {PAGED_HEAD}], got {list(k_pages.shape)}")
-    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or not v_pages.is_contiguous():
-        raise SpnError(f"{name}: v_pages must be like k_pages")
-    return k_pages.shape[:3]
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor) -> None:
@@ -1540,17 +1548,19 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     _paged_size(n, page)
     _paged_check(n, k_pages.data_ptr() != v_pages.data_ptr(), "k_pages and v_pages are the same memory")
     T = slots.numel()
-    for arg, t in (("k", k), ("v", v)):
-        if t.shape != (T, kvh, PAGED_HEAD) or t.stride(2) != 1:
-            raise SpnError(f"{n}: {arg} must be [{T}, {kvh}, {PAGED_HEAD}] with unit inner stride, got {list(t.shape)}")
-    _paged_check(n, k.dtype == v.dtype, "k and v must have one dtype")
+    want, ks, vs = (T, kvh, PAGED_HEAD), k.stride(), v.stride()
+    if k.shape != want or ks[2] != 1:
+        raise SpnError(f"{n}: k must be {list(want)} with unit inner stride, got {list(k.shape)}")
+    if v.shape != want or vs[2] != 1:
+        raise SpnError(f"{n}: v must be {list(want)} with unit inner stride, got {list(v.shape)}")
+    _paged_check(n, k.dtype is v.dtype, "k and v must have one dtype")
     rd, pd = _dt(k), _dt(k_pages)
-    _paged_check(n, slots.dtype == torch.int64 and slots.is_contiguous(), "slots must be contiguous int64")
-    _paged_check(n, T * kvh < 2 ** 28, "rows x heads stay under 2^28")
+    _paged_check(n, slots.dtype is torch.int64 and slots.is_contiguous(), "slots must be contiguous int64")
+    _paged_check(n, T * kvh < 2 ** 26, "rows x heads stay under 2^26")
     dev = _paged_device(n, k, v, k_pages, v_pages, slots)
     if T == 0:
         return
-    _paged_call(dev, "spn_paged_append", k.data_ptr(), v.data_ptr(), rd, k.stride(0), k.stride(1), v.stride(0), v.stride(1), k_pages.data_ptr(),
+    _paged_call(dev, "spn_paged_append", k.data_ptr(), v.data_ptr(), rd, ks[0], ks[1], vs[0], vs[1], k_pages.data_ptr(),
                 v_pages.data_ptr(), pd, slots.data_ptr(), T, kvh, num_pages, page)
 
 
@@ -1567,24 +1577,27 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     n = "paged_attn"
     num_pages, kvh, page = _paged_pools(n, k_pages, v_pages)
     R, W, ld = _paged_table(n, block_table, page)
-    if q.ndim != 3 or q.shape[0] != R or q.shape[2] != PAGED_HEAD or q.stride(2) != 1 or q.dtype != k_pages.dtype:
-        raise SpnError(f"{n}: q must be {k_pages.dtype} [{R}, heads, {PAGED_HEAD}] with unit inner stride, got {q.dtype} {list(q.shape)}")
-    h, dt = q.shape[1], _dt(q)
-    _paged_check(n, h > 0 and h % kvh == 0, f"{h} heads on {kvh} key heads")
-    _paged_ints(n, "lens", lens, (R,))
-    if slopes is not None and (slopes.dtype != F32 or slopes.shape != (h,) or not slopes.is_contiguous()):
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 3 or shape[0] != R or shape[2] != PAGED_HEAD or strides[2] != 1 or q.dtype is not k_pages.dtype:
+        raise SpnError(f"{n}: q must be {k_pages.dtype} [{R}, heads, {PAGED_HEAD}] with unit inner stride, got {q.dtype} {list(shape)}")
+    h, dt = shape[1], _dt(q)
+    if h < 1 or h % kvh or R * h >= 2 ** 21:
+        raise SpnError(f"{n}: {h} heads on {kvh} key heads for {R} requests (a multiple of the key heads; requests x heads stay under 2^21)")
+    _paged_ints(n, "lens", lens, R)
+    if slopes is not None and (slopes.dtype is not F32 or slopes.shape != (h,) or not slopes.is_contiguous()):
         raise SpnError(f"{n}: slopes must be contiguous fp32 [{h}]")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or (h > 1 and out.stride(1) < PAGED_HEAD)
                             or (R > 1 and out.stride(0) < (h - 1) * out.stride(1) + PAGED_HEAD)):
         raise SpnError(f"{n}: out must be like q with unit inner stride and rows that do not overlap")
     dev = _paged_device(n, q, k_pages, v_pages, block_table, lens, slopes, out)
     if out is None:
-        out = torch.empty((R, h, PAGED_HEAD), device=dev, dtype=q.dtype)
+        out = torch.empty(shape, device=dev, dtype=q.dtype)
     if R == 0:
         return out
+    o_rs, o_hs, _ = out.stride()
     ws_bytes = load().spn_paged_attn_workspace_bytes(R, h, kvh, W, page, dt)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
-    _paged_call(dev, "spn_paged_attn", q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(), dt, block_table.data_ptr(),
-                ld, lens.data_ptr(), None if slopes is None else slopes.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), R, h,
+    _paged_call(dev, "spn_paged_attn", q.data_ptr(), strides[0], strides[1], k_pages.data_ptr(), v_pages.data_ptr(), dt, block_table.data_ptr(),
+                ld, lens.data_ptr(), None if slopes is None else slopes.data_ptr(), out.data_ptr(), o_rs, o_hs, R, h,
                 kvh, W, num_pages, page, PAGED_HEAD ** -0.5 if scale is None else float(scale), None if ws is None else ws.data_ptr(), ws_bytes)
     return out
