@@ -106,7 +106,14 @@ class TupleTransformer(nn.Module, Constructor):
                 context: Optional[Tensor] = None, context_mask: Optional[Tensor] = None,
                 caches: Optional[TupleTransformerCaches] = None, logits_keys: Optional[List] = None,
                 return_embeddings: bool = False, return_attn: bool = False, return_caches: bool = False,
-                labels: Optional[Tensor] = None, want_argmax: bool = False, label_counts=None, **kwargs):
+                labels: Optional[Tensor] = None, want_argmax: bool = False, label_counts=None, paged=None, **kwargs):
+        """`paged`: a step of a PagedKVCache made for `self.transformer`; x [R, width, dims] are the new notes of every request, context / style
+        embeddings theirs alone.  The caches of the reference's protocol (`caches`, `return_caches`) do not go with it."""
+        if paged is not None:
+            if caches is not None or return_caches or mask is not None:
+                raise ValueError("a paged step brings its own mask and cache")
+            if self.pos_emb is not None:
+                raise NotImplementedError("paged steps with absolute position embeddings: the notes' positions are on the device")
         token_emb_cache = caches.token_emb if caches is not None else None
         if hasattr(self.token_emb, "multiseq_mode") and x_extra is not None:
             x_extra = [x_extra] if isinstance(x_extra, Tensor) else x_extra
@@ -140,7 +147,7 @@ class TupleTransformer(nn.Module, Constructor):
         out, intermediates = self.transformer(
             x, mask=mask.contiguous() if mask is not None else None, context=context, context_mask=context_mask,
             style_embeddings=style_embeddings, intermediates_cache=caches.transformer if caches is not None else None,
-            return_hiddens=True)
+            return_hiddens=True, paged=paged)
 
         logits = ce_sums = argmax = eval_sums = None
         if not return_embeddings and self.lm_head is not None:

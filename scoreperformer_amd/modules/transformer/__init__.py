@@ -5,6 +5,7 @@ from .embeddings import (
     FixedPositionalEmbedding, ALiBiPositionalBias, LearnedALiBiPositionalBias
 )
 from .feedforward import FeedForwardConfig, FeedForward
+from .paged import PagedKVCache, PagedStep
 from .transformer import (
     TransformerIntermediates, TransformerRegistry, TransformerConfig, Transformer,
     EncoderConfig, Encoder, DecoderConfig, Decoder

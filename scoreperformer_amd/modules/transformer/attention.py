@@ -12,6 +12,7 @@ Options of the reference class beyond the shipped recipes:
   visible (the key mask is padded with True, causal masks start behind them), positions shifted by their number in the ALiBi bias
   exactly as `rel_pos.get_bias(i, j, k=j - i)` shifts them.  Multi-head K/V only: with `one_kv_head` the reference itself fails in
   `torch.cat((mem_k, k))` ([b, h, m, d] against [b, n, d]).
+* `paged` (a PagedStep, layer index): the keys / values of earlier rows live in a PagedKVCache instead of `cache` (paged.py); inference only.
 * `max_attend` (attention.py:170-187) raises: the reference's mask `(-max_attend < dist) | (dist > max_attend)` is true for every
   key except those at least `max_attend` positions in a query's FUTURE -- with `causal` every score is masked -- so there is no
   behaviour worth reproducing; no recipe sets it.
@@ -129,11 +130,36 @@ class Attention(nn.Module, Constructor):
         mem = F_.cast(torch.cat([rows(self.mem_k), rows(self.mem_v)], dim=-1), torch.bfloat16)
         return mem[None].expand(b, -1, -1)
 
+    def _paged(self, x: Tensor, step, layer: int, residual: Optional[Tensor]):
+        """The rows of a paged step: appended to the layer's pages; single rows attend over the pages, prompts over themselves (the dense kernel)."""
+        b, n = x.shape[:2]
+        h, kvh = self.heads, self.kv_heads
+        if torch.is_grad_enabled() or self.training:
+            raise RuntimeError("the paged cache serves inference: call under torch.no_grad() in eval mode")
+        if not self.causal or self.num_mem_kv > 0 or kvh != step.cache.kv_heads or (b, n) != tuple(step.slots.shape):
+            raise ValueError(f"rows {(b, n)} of a {'' if self.causal else 'non-'}causal layer with {kvh} key heads do not fit the paged step "
+                             f"{tuple(step.slots.shape)} over {step.cache.kv_heads} key heads")
+        qkv = F_.linear(x, self._fused("_w_qkv", (self.to_q.weight, self.to_k.weight, self.to_v.weight)))
+        slopes = self.rel_pos.padded_slopes() if self.rel_pos is not None else None
+        q, k, v = (t.unflatten(-1, (-1, 64)) for t in qkv.view(b * n, -1).split((h * 64, kvh * 64, kvh * 64), dim=-1))
+        step.cache.append(layer, k, v, step)
+        if n == 1:
+            sl = slopes.reshape(-1).float().contiguous() if slopes is not None else None
+            o = step.cache.attend(layer, q, step, self.scale, sl).view(b, 1, h * 64)
+        else:
+            o = F_.SelfAttnFn.apply(qkv, slopes, step.mask, h, kvh, True, self.scale, 0.0, step.mask)
+        out = F_.linear(o, self._head_cols(self.to_out.weight), residual=residual, rowmask=step.mask, out_fp32=residual is not None)
+        return out, AttentionIntermediates(), AttentionSharedIntermediates(rel_pos_bias=None)
+
     @no_autocast
     def forward(self, x: Tensor, context: Optional[Tensor] = None, mask: Optional[Tensor] = None,
                 context_mask: Optional[Tensor] = None, attn_mask: Optional[Tensor] = None, prev_attn: Optional[Tensor] = None,
                 mem: Optional[Tensor] = None, cache: Optional[AttentionIntermediates] = None,
-                shared_cache: Optional[AttentionSharedIntermediates] = None, residual: Optional[Tensor] = None):
+                shared_cache: Optional[AttentionSharedIntermediates] = None, residual: Optional[Tensor] = None, paged=None):
+        if paged is not None:
+            if context is not None or mask is not None or context_mask is not None or attn_mask is not None or mem is not None or cache is not None:
+                raise ValueError("a paged step brings its own mask and keys: no context, mask, memory or cache beside it")
+            return self._paged(x, *paged, residual)
         b, n = x.shape[:2]
         h, kvh = self.heads, self.kv_heads
         has_context, has_mem, has_cache = context is not None, mem is not None, cache is not None

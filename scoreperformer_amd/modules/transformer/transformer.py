@@ -17,6 +17,7 @@ from ..layers import Residual, AdaptiveLayerNorm, LayerNorm
 from .attend import AttentionIntermediates
 from .attention import Attention, AttentionConfig
 from .feedforward import FeedForward, FeedForwardConfig
+from .paged import PagedStep
 from ...utils.amp import no_autocast
 
 
@@ -88,7 +89,15 @@ class Transformer(nn.Module, Constructor):
     def forward(self, x: Tensor, mask: Optional[Tensor] = None, context: Optional[Tensor] = None,
                 context_mask: Optional[Tensor] = None, attn_mask: Optional[Tensor] = None,
                 style_embeddings: Optional[Tensor] = None, mems: Optional[List[Tensor]] = None,
-                intermediates_cache: Optional[TransformerIntermediates] = None, return_hiddens: bool = False):
+                intermediates_cache: Optional[TransformerIntermediates] = None, return_hiddens: bool = False,
+                paged: Optional[PagedStep] = None):
+        """`paged`: a step of a PagedKVCache made for this stack -- x holds the new rows of every request [R, width, dim]; rows without a slot
+        are padding (no `mask` beside it)."""
+        if paged is not None and (mask is not None or intermediates_cache is not None or self.cross_attend):
+            raise ValueError("a paged step brings its own mask and cache")
+        if paged is not None and paged.cache.num_layers != self.num_attn_layers:
+            raise ValueError(f"a paged step over {paged.cache.num_layers} layers for a stack of {self.num_attn_layers}")
+        layer_index = 0
         assert not (self.cross_attend ^ (context is not None)), 'context must be passed in if cross_attend is set to True'
         assert not self.ada_norm or style_embeddings is not None, 'style_embeddings must be passed for AdaLayerNorm'
         if mems is not None or attn_mask is not None:
@@ -127,7 +136,10 @@ class Transformer(nn.Module, Constructor):
                 h = self._norm(pre_norm, x, style_embeddings) if pre_norm is not None else F_.cast(x, torch.bfloat16)
             fuse = residual_fn.is_plain
             res_arg = residual if fuse else None
-            if layer_type == 'a':
+            if layer_type == 'a' and paged is not None:
+                out, inter, _ = block(h, residual=res_arg, paged=(paged, layer_index))
+                layer_index += 1
+            elif layer_type == 'a':
                 out, inter, _ = block(h, mask=mask, cache=cache, residual=res_arg)
             elif layer_type == 'c':
                 # under the cache protocol the block sees ONE query: its row mask is the last column.  (The reference passes the

@@ -176,3 +176,47 @@ def test_attention_oracle_is_softmax_attention_of_the_gathered_rows():
         s = torch.einsum("hjd,hd->hj", k, q[r].double()) / 8 + slopes.double()[:, None] * torch.arange(-n + 1, 1).double()
         want = torch.einsum("hj,hjd->hd", torch.exp(s) / torch.exp(s).sum(1, keepdim=True), v)
         assert (got[r] - want).abs().max() < 1e-12
+
+
+def _stack(**kw):
+    from scoreperformer_amd.modules.transformer import Decoder
+    return Decoder(dim=64, depth=2, heads=1, **kw).eval()
+
+
+def test_paged_cache_refuses_what_it_does_not_serve():
+    from scoreperformer_amd.modules.transformer import AttentionConfig, Encoder, PagedKVCache
+    ok = dict(num_pages=4, max_requests=2, max_len=20)
+    c = PagedKVCache(_stack(), **ok)
+    assert c.k_pages.shape == (2, 4, 1, 16, 64) and c.block_table.shape == (2, 2) and int(c.num_free) == 4 and c.k_pages.dtype == torch.bfloat16
+    with pytest.raises(NotImplementedError, match="causal"):
+        PagedKVCache(Encoder(dim=64, depth=2, heads=1), **ok)
+    with pytest.raises(NotImplementedError, match="cross"):
+        PagedKVCache(_stack(cross_attend=True), **ok)
+    with pytest.raises(NotImplementedError, match="memory"):
+        PagedKVCache(_stack(attention=AttentionConfig(num_mem_kv=2)), **ok)
+    for bad in (dict(num_pages=0), dict(max_requests=0), dict(max_len=0), dict(page_size=12), dict(page_size=4)):
+        with pytest.raises(ValueError):
+            PagedKVCache(_stack(), **{**ok, **bad})
+
+
+def test_paged_steps_refuse_masks_gradients_and_other_stacks():
+    from scoreperformer_amd.modules.transformer import AttentionConfig, PagedKVCache, PagedStep
+    stack = _stack(attention=AttentionConfig(one_kv_head=True))
+    cache = PagedKVCache(stack, num_pages=4, max_requests=2, max_len=20)
+    step = PagedStep(cache, torch.zeros(2, 1, dtype=torch.int64), torch.ones(2, 1, dtype=torch.bool), torch.ones(2, dtype=torch.int32))
+    x = torch.zeros(2, 1, 64)
+    with pytest.raises(ValueError, match="own mask"):
+        stack(x, mask=torch.ones(2, 1, dtype=torch.bool), paged=step)
+    with pytest.raises(ValueError, match="layers"):
+        _stack().__class__(dim=64, depth=3, heads=1)(x, paged=step)
+    attn = stack.layers[0][1]
+    with pytest.raises(ValueError, match="no context"):
+        attn(x, mask=step.mask, paged=(step, 0))
+    with pytest.raises(RuntimeError, match="inference"):
+        attn(x, paged=(step, 0))
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="do not fit"):
+            attn(torch.zeros(3, 1, 64), paged=(step, 0))
+        attn.train()
+        with pytest.raises(RuntimeError, match="inference"):
+            attn(x, paged=(step, 0))
