@@ -83,6 +83,7 @@ __global__ __launch_bounds__(PLAN_T) void plan_kernel(PlanArgs a) {
         __syncthreads();
         carry += red[0];
         if (FILL) {
+#pragma unroll 4
             for (int e = tid; e < n * a.width; e += PLAN_T) {   // at most FILL_ONE
                 const int q = e / a.width, i = e - q * a.width;
                 plan_emit(a, r0 + q, i, s_len[q], s_given[q], s_top[q]);
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(PLAN_T) void plan_kernel(PlanArgs a) {
     if (tid == 0) *a.num_free_out = nf - s_taken;
 }
 
-constexpr int FILL_ONE = 4096;   // slots up to which one workgroup fills them itself: four a thread; a second launch costs as much
+constexpr int FILL_ONE = 8192;   // slots up to which one workgroup fills them itself (64 x 128: 9.5 us; in two launches 8.3, and 4 us more of host time; 64 x 256: 13.7)
 constexpr int FILL_B = 1024;     // slots of a workgroup of the second launch
 
 __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a) {

@@ -247,6 +247,41 @@ def test_attention_matches_the_oracle(dev, dtype, heads, which, page, bias):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kvh, lens, page", [(8, [(i * 53) % 901 for i in range(40)], 16),           # whole segments: 4 waves each
+                                             (8, [(i * 311) % 2101 for i in range(33)], 8),           # 8 waves, long tables
+                                             (8, [4096 - (i * 331) % 4096 for i in range(36)], 64),    # 8 waves, rows not kept in the caches
+                                             (1, [70001], 32), (1, [131, 40000, 7], 16),               # cut: many parts of one request
+                                             (4, [20000, 0, 39999, 25000], 128)])                      # cut, rows not kept in the caches
+def test_attention_of_large_batches_matches_the_oracle(dev, dtype, kvh, lens, page):
+    """The sizes at which the work is divided and the rows are read in other ways."""
+    kp, vp, table, lens = _cache(dev, lens, kvh, page, dtype, seed=7)
+    q = torch.randn(len(lens), 8, 64, generator=torch.Generator().manual_seed(2)).to(dtype)
+    _check(dev, q, kp, vp, table, lens, _slopes(8) / 64)      # shallow slopes: far rows count
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("scale", [0.0, 1e-30, -0.125, 1e-12, 3.0])
+def test_attention_with_any_scale(dev, dtype, scale):
+    kp, vp, table, lens = _cache(dev, [300, 5, 0], 2, 8, dtype)
+    q = torch.randn(3, 6, 64).to(dtype)
+    got = _ops().paged_attn(q.to(dev), kp.to(dev), vp.to(dev), table.to(dev), lens.to(dev), scale=scale, slopes=_slopes(6).to(dev))
+    want = paged_cpu.attn(q, kp, vp, table, lens, scale, _slopes(6))
+    assert bool(((got.cpu().double() - want).abs() <= _tolerance(q, kp, vp, table, lens, _slopes(6), abs(scale), want)).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_in_place_of_its_query_and_over_a_slice_of_a_wider_table(dev, dtype):
+    kp, vp, table, lens = _cache(dev, [700, 31, 0, 2500], 2, 16, dtype)
+    wide = torch.full((4, table.shape[1] + 9), 2 ** 31 - 1, dtype=torch.int32)
+    wide[:, 4:4 + table.shape[1]] = table
+    q = torch.randn(4, 4, 64).to(dtype)
+    want = _ops().paged_attn(q.to(dev), kp.to(dev), vp.to(dev), table.to(dev), lens.to(dev))
+    d_q = q.to(dev)
+    got = _ops().paged_attn(d_q, kp.to(dev), vp.to(dev), wide.to(dev)[:, 4:4 + table.shape[1]], lens.to(dev), out=d_q)
+    assert got is d_q and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_attention_strides_scale_and_given_output(dev, dtype):
     """q as a slice of the fused projection, heads in front; the output into a slice of a wider buffer, nothing beside it touched."""
     kp, vp, table, lens = _cache(dev, [40, 3, 77], 2, 16, dtype)
