@@ -353,7 +353,8 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
 
-template <typename T> __device__ __forceinline__ int tiles_of(const PagedAttnArgs& a, int r) { return (rows_of(a.lens[r], a.W, a.shift) + TILE<T> - 1) / TILE<T>; }
+template <typename T> __device__ __forceinline__ int tiles_in(int rows) { return (rows + TILE<T> - 1) / TILE<T>; }
+__device__ __forceinline__ int rows_at(const PagedAttnArgs& a, int r) { return rows_of(a.lens[r], a.W, a.shift); }
 
 // parts of a segment of `tiles` tiles, none above `most` tiles unless there would be more than MAX_PARTS
 __device__ __forceinline__ int parts_of(int tiles, int most) { return max(1, min(MAX_PARTS, (int)(((uint32_t)tiles + (uint32_t)most - 1u) / (uint32_t)most))); }
@@ -369,22 +370,23 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(PagedAttnArgs
     __shared__ __attribute__((aligned(1024))) char smem[WAVES][2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), H = a.kvh * a.passes;
     const int wg = blockIdx.x;
-    int r, hp, part = 0, parts = 1;
+    int r, n, hp, part = 0, parts = 1;
     bool once = a.once;
     if constexpr (DIRECT) {
         r = wg / H; hp = wg - r * H;
+        n = rows_at(a, r);
     } else {
         const int per = (a.R + 63) / 64, q0 = min(a.R, lane * per), q1 = min(a.R, q0 + per);   // this lane's requests
-        const int first = q0 < q1 ? tiles_of<T>(a, q0) : 0;
-        long mine = first;
-        for (int q = q0 + 1; q < q1; ++q) mine += tiles_of<T>(a, q);
+        const int first = q0 < q1 ? rows_at(a, q0) : 0;
+        long mine = tiles_in<T>(first);
+        for (int q = q0 + 1; q < q1; ++q) mine += tiles_in<T>(rows_at(a, q));
         // in two halves of 32 bits: table capacities pass 2^32 tiles before memory does
         const long total = H * (((long)__builtin_amdgcn_readlane(wave_scan((int)(mine >> 16)), 63) << 16) +
                                 (uint32_t)__builtin_amdgcn_readlane(wave_scan((int)(mine & 0xffff)), 63));
         const int most = (int)min(max((long)MIN_TILES, (total + TARGET - 1) / TARGET), (long)a.max_tiles);
         once = total * STAGE >= ONCE;
-        int units = q0 < q1 ? H * parts_of(first, most) : 0;
-        for (int q = q0 + 1; q < q1; ++q) units += H * parts_of(tiles_of<T>(a, q), most);
+        int units = q0 < q1 ? H * parts_of(tiles_in<T>(first), most) : 0;
+        for (int q = q0 + 1; q < q1; ++q) units += H * parts_of(tiles_in<T>(rows_at(a, q)), most);
         const int incl = wave_scan(units);
         const unsigned long long behind = __ballot(incl > wg);
         if (!behind) {
@@ -394,15 +396,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(PagedAttnArgs
         const int at = __builtin_ctzll(behind);
         int off = wg - __builtin_amdgcn_readlane(incl - units, at);
         r = at * per;
+        n = __builtin_amdgcn_readlane(first, at);
         for (;;) {
-            parts = parts_of(tiles_of<T>(a, r), most);
+            parts = parts_of(tiles_in<T>(n), most);
             if (off < H * parts) break;
-            off -= H * parts; ++r;
+            off -= H * parts;
+            n = rows_at(a, ++r);   // (a lane's later requests: more than 64 in the batch)
         }
         hp = off / parts; part = off - hp * parts;
     }
-    r = __builtin_amdgcn_readfirstlane(r);
-    const int n = rows_of(a.lens[r], a.W, a.shift), tiles = (n + TILE<T> - 1) / TILE<T>;
+    const int tiles = tiles_in<T>(n);
     const int t0 = DIRECT ? 0 : (int)((long)tiles * part / parts), t1 = DIRECT ? tiles : (int)((long)tiles * (part + 1) / parts);
     const int kh = hp / a.passes, first = (hp - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
     Walk<T, WAVES> wk(a, lane, smem[w]);
