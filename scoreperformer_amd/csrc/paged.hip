@@ -150,7 +150,7 @@ __global__ __launch_bounds__(PLAN_T) void release_kernel(ReleaseArgs a) {
             const bool ok = page_ok(id, a.num_pages);
             const unsigned long long m = __ballot(ok);
             const long to = at - __popcll(m & ((1ull << lane) - 1));
-            if (ok && to < a.num_pages) a.stack[to] = id;      // past the end: more pages come back than the pool has, one was held twice
+            if (ok && to >= 0 && to < a.num_pages) a.stack[to] = id;      // past the end: more pages come back than the pool has, one was held twice
             if (j + lane < held) a.table[r * a.ld + j + lane] = -1;
             at -= __popcll(m);
         }

@@ -399,11 +399,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(PagedAttnArgs
         n = __builtin_amdgcn_readlane(first, at);
         for (;;) {
             parts = parts_of(tiles_in<T>(n), most);
-            if (off < H * parts) break;
+            if (off < H * parts || r + 1 >= a.R) break;
             off -= H * parts;
             n = rows_at(a, ++r);   // (a lane's later requests: more than 64 in the batch)
         }
-        hp = off / parts; part = off - hp * parts;
+        // (the bounds hold by themselves unless the lengths change while this runs; then the result is lost, but no access goes astray)
+        hp = min(off / parts, H - 1); part = min(off - hp * parts, parts - 1);
     }
     const int tiles = tiles_in<T>(n);
     const int t0 = DIRECT ? 0 : (int)((long)tiles * part / parts), t1 = DIRECT ? tiles : (int)((long)tiles * (part + 1) / parts);

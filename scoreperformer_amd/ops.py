@@ -1463,23 +1463,22 @@ def _paged_pools(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor) -> Tup
     return n, kvh, page
 
 
-def _paged_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
-    """All tensors on one GPU; returns it."""
+def _paged_device(name: str, *tensors: Optional[torch.Tensor]) -> int:
+    """All tensors on one GPU; returns its number."""
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != index or index < 0:
             require_gpu(*tensors)
             raise SpnError(f"{name}: tensors on {tensors[0].device} and {t.device}")
-    return tensors[0].device
+    return index
 
 
-def _paged_call(dev: torch.device, fn: str, *args) -> None:
-    """The call on the current stream of `dev`, whichever device is current."""
-    index = dev.index
+def _paged_call(index: int, fn: str, *args) -> None:
+    """The call on the current stream of GPU `index`, whichever device is current."""
     if index == torch.cuda.current_device():
         call(fn, *args, raw_stream(index))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             call(fn, *args, raw_stream(index))
 
 
@@ -1506,14 +1505,14 @@ def paged_plan(lens: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor,
         _paged_ints(n, "num_free_out", num_free_out, 1)
     _paged_check(n, width >= 1 and R * width < 2 ** 31, "width must be at least 1, requests x width under 2^31")
     dev = _paged_device(n, lens, new, block_table, free_pages, num_free, lens_out, num_free_out)
-    slots = torch.empty((R, width), device=dev, dtype=torch.int64)
+    slots = lens.new_empty((R, width), dtype=torch.int64)
     lens_out = torch.empty_like(lens) if lens_out is None else lens_out
     num_free_out = torch.empty_like(num_free) if num_free_out is None else num_free_out
     if R == 0:
         num_free_out.copy_(num_free)
         return slots, lens_out, num_free_out
     ws_bytes = load().spn_paged_plan_workspace_bytes(R, width) if R * width > 1024 else 0   # (never for fewer slots)
-    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+    ws = lens.new_empty(ws_bytes // 4) if ws_bytes else None
     _paged_call(dev, "spn_paged_plan", lens.data_ptr(), new.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(),
                 num_free.data_ptr(), lens_out.data_ptr(), num_free_out.data_ptr(), slots.data_ptr(), R, W, free_pages.numel(), page_size, width,
                 None if ws is None else ws.data_ptr(), ws_bytes)
@@ -1534,7 +1533,7 @@ def paged_release(done: torch.Tensor, lens: torch.Tensor, block_table: torch.Ten
     dev = _paged_device(n, done, lens, block_table, free_pages, num_free)
     if R == 0:
         return
-    ws = torch.empty(R + 1, device=dev, dtype=torch.int32)
+    ws = lens.new_empty(R + 1)
     _paged_call(dev, "spn_paged_release", done.data_ptr(), lens.data_ptr(), block_table.data_ptr(), ld, free_pages.data_ptr(),
                 num_free.data_ptr(), R, W, free_pages.numel(), page_size, ws.data_ptr())
 
@@ -1587,17 +1586,19 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     _paged_ints(n, "lens", lens, R)
     if slopes is not None and (slopes.dtype is not F32 or slopes.shape != (h,) or not slopes.is_contiguous()):
         raise SpnError(f"{n}: slopes must be contiguous fp32 [{h}]")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or (h > 1 and out.stride(1) < PAGED_HEAD)
-                            or (R > 1 and out.stride(0) < (h - 1) * out.stride(1) + PAGED_HEAD)):
-        raise SpnError(f"{n}: out must be like q with unit inner stride and rows that do not overlap")
+    if out is not None:
+        (o_rs, o_hs, inner), d = out.stride(), PAGED_HEAD
+        apart = ((h == 1 or o_hs >= d) and (R == 1 or o_rs >= (h - 1) * o_hs + d)) or ((R == 1 or o_rs >= d) and (h == 1 or o_hs >= (R - 1) * o_rs + d))
+        if out.shape != shape or out.dtype is not q.dtype or inner != 1 or not (apart or R == 0):
+            raise SpnError(f"{n}: out must be like q, with unit inner stride and rows that do not overlap")
     dev = _paged_device(n, q, k_pages, v_pages, block_table, lens, slopes, out)
     if out is None:
-        out = torch.empty(shape, device=dev, dtype=q.dtype)
+        out = q.new_empty(shape)
     if R == 0:
         return out
     o_rs, o_hs, _ = out.stride()
     ws_bytes = load().spn_paged_attn_workspace_bytes(R, h, kvh, W, page, dt)
-    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+    ws = lens.new_empty(ws_bytes // 4) if ws_bytes else None   # (a multiple of 4 bytes)
     _paged_call(dev, "spn_paged_attn", q.data_ptr(), strides[0], strides[1], k_pages.data_ptr(), v_pages.data_ptr(), dt, block_table.data_ptr(),
                 ld, lens.data_ptr(), None if slopes is None else slopes.data_ptr(), out.data_ptr(), o_rs, o_hs, R, h,
                 kvh, W, num_pages, page, PAGED_HEAD ** -0.5 if scale is None else float(scale), None if ws is None else ws.data_ptr(), ws_bytes)

@@ -294,6 +294,7 @@ def test_attention_strides_scale_and_given_output(dev, dtype):
     assert got.data_ptr() == out[:, 2:6, 3:67].data_ptr()
     out[:, 2:6, 3:67] = 7.0
     assert bool((out == 7).all())
+    _check(dev, q, kp, vp, table, lens, out=torch.empty(4, 3, 64, device=dev, dtype=dtype).transpose(0, 1))      # heads in front
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
