@@ -69,17 +69,35 @@ __device__ __forceinline__ float max3(float a, float b, float c) {   // without 
     return r;
 }
 
-// LDS DMA: 16 bytes per lane from base + off(lane) into LDS [lds .. lds + 1023], lane-major (common.h spn_dma16, with a 64-bit base instead of a
-// buffer resource: a pool passes 4 GiB).  The compiler does not count it: whoever reads waits by hand.  NT: not kept in the caches.
-template <bool NT>
-__device__ __forceinline__ void dma16(uint32_t lds, uint32_t off, const char* base) {
-    if constexpr (NT) asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" :: "s"(lds), "v"(off), "s"(base) : "memory");
-    else asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
+// LDS DMA of N consecutive KiB: 16 bytes per lane and piece, piece k from base + 1024 k + off[k](lane) into LDS [lds + 1024 k ..), lane-major
+// (common.h spn_dma16, with a 64-bit base instead of a buffer resource: a pool passes 4 GiB; the instruction's offset counts on both sides).  The
+// compiler does not count it: whoever reads waits by hand.  NT: not kept in the caches.
+template <int N, bool NT>
+__device__ __forceinline__ void dma(uint32_t lds, const uint32_t* off, const char* base) {
+#define SPN_LEAD "s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\t"
+    if constexpr (N == 1) {
+        if constexpr (NT) asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %2 nt" :: "s"(lds), "v"(off[0]), "s"(base) : "memory");
+        else asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off[0]), "s"(base) : "memory");
+    } else if constexpr (N == 2) {
+        if constexpr (NT)
+            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %3 nt\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024 nt"
+                         :: "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
+        else asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" :: "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
+    } else {
+        static_assert(N == 4, "pieces of one base");
+        if constexpr (NT)
+            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %5 nt\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024 nt\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048 nt\n\t"
+                         "global_load_lds_dwordx4 %4, %5 offset:3072 nt" :: "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory");
+        else
+            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+                         "global_load_lds_dwordx4 %4, %5 offset:3072" :: "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory");
+    }
+#undef SPN_LEAD
 }
 
-// The page ids of a tile's groups of 8 rows (a page holds at least 8): the same for all lanes, so they come by scalar loads -- off the counter of
-// the vector loads -- and are checked by scalar instructions.
-template <typename T> struct Pages { int id[TILE<T> / 8]; bool ok[TILE<T> / 8]; };
+// The page ids of a tile's groups of UNIT rows (8 where pages have 8, else 16): the same for all lanes, so they come by scalar loads -- off the
+// counter of the vector loads -- and are checked by scalar instructions.
+template <typename T, int UNIT> struct Pages { static constexpr int N = TILE<T> / UNIT; int id[N]; uint32_t bad; };   // bad: bit c, group c lies on no page
 
 // One wave's walk over some tiles of one segment: the state of the softmax of 16 heads, a head per lane & 15.  Lane (i = lane & 15, g = lane >> 4).
 // E: rows of a tile that a lane holds scores of.  bf16: tile rows 8 g + 0 .. 7 (row i of score product t is tile row (i >> 2) * 8 + 4 t + (i & 3),
@@ -166,40 +184,47 @@ struct Walk {
     }
 
     // rows outside the request count as its first or last one: their loads stay on its pages, their scores are dropped
-    __device__ __forceinline__ Pages<T> pages(int t) const {
+    template <int UNIT> __device__ __forceinline__ Pages<T, UNIT> pages(int t) const {
         const uint32_t at = (uint32_t)max(t, 0) * TILE<T>, last = (uint32_t)(n - 1) >> a.shift;
-        Pages<T> p;
+        Pages<T, UNIT> p;
+        p.bad = 0;
 #pragma unroll
-        for (int c = 0; c < TILE<T> / 8; ++c) p.id[c] = trow[min((at + 8 * c) >> a.shift, last)];
+        for (int c = 0; c < p.N; ++c) p.id[c] = trow[min((at + UNIT * c) >> a.shift, last)];
         return p;
     }
-    // an entry that is no page: page 0's rows, masked by `ok`
-    __device__ __forceinline__ void check(Pages<T>& p) const {
+    // an entry that is no page: page 0's rows, masked by `bad`
+    template <int UNIT> __device__ __forceinline__ void check(Pages<T, UNIT>& p) const {
 #pragma unroll
-        for (int c = 0; c < TILE<T> / 8; ++c) { p.ok[c] = page_ok(p.id[c], a.num_pages); p.id[c] = p.ok[c] ? p.id[c] : 0; }
+        for (int c = 0; c < p.N; ++c) {
+            const bool ok = page_ok(p.id[c], a.num_pages);
+            p.bad |= ok ? 0u : 1u << c;
+            p.id[c] = ok ? p.id[c] : 0;
+        }
     }
-    template <bool NT>
-    __device__ __forceinline__ void fetch(int t, const Pages<T>& p, uint32_t stage) const {
-        constexpr int PIECE = 1024 / ROW;   // rows of a piece, inside one group of 8
+    template <int UNIT, bool NT>
+    __device__ __forceinline__ void fetch(int t, const Pages<T, UNIT>& p, uint32_t stage) const {
+        constexpr int PIECES = UNIT * ROW / 1024;
         const uint32_t mask = (1u << a.shift) - 1u;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint64_t at = (uint64_t)(uint32_t)p.id[q * PIECE / 8] * page_bytes + (((uint32_t)t * TILE<T> + PIECE * q) & mask) * ROW;
-            dma16<NT>(lds0 + stage + q * 1024, off[q], kb + at);
-            dma16<NT>(lds0 + stage + 4096 + q * 1024, off[q], vb + at);
+        for (int c = 0; c < p.N; ++c) {
+            // (uniform by construction; said once more, because the compiler does not always see it through the loop)
+            const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane(p.id[c]) * page_bytes +
+                                (uint32_t)__builtin_amdgcn_readfirstlane((((uint32_t)t * TILE<T> + UNIT * c) & mask) * ROW);
+            dma<PIECES, NT>(lds0 + stage + c * PIECES * 1024, off + c * PIECES, kb + at);
+            dma<PIECES, NT>(lds0 + stage + 4096 + c * PIECES * 1024, off + c * PIECES, vb + at);
         }
     }
 
     // Tiles t, t - WAVES, ... down to t0, the newest rows first.  Two tiles are on their way while one is computed; a tile's LDS is refilled as soon
     // as it has been read into registers.
-    template <bool NT>
+    template <int UNIT, bool NT>
     __device__ __forceinline__ void run(int t, int t0) {
         if (t < t0) return;
-        Pages<T> now = pages(t), next = pages(t - WAVES), then = pages(t - 2 * WAVES);
+        Pages<T, UNIT> now = pages<UNIT>(t), next = pages<UNIT>(t - WAVES), then = pages<UNIT>(t - 2 * WAVES);
         check(now);
-        fetch<NT>(t, now, 0);
+        fetch<UNIT, NT>(t, now, 0);
         check(next);
-        if (t - WAVES >= t0) fetch<NT>(t - WAVES, next, STAGE);
+        if (t - WAVES >= t0) fetch<UNIT, NT>(t - WAVES, next, STAGE);
         uint32_t stage = 0;
         for (;;) {
             const bool more = t - WAVES >= t0;
@@ -236,9 +261,9 @@ struct Walk {
             check(then);
             if (t - 2 * WAVES >= t0) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this tile has been read
-                fetch<NT>(t - 2 * WAVES, then, stage);
+                fetch<UNIT, NT>(t - 2 * WAVES, then, stage);
             }
-            const Pages<T> later = pages(t - 3 * WAVES);   // behind the LDS reads: scalar loads share their counter
+            const Pages<T, UNIT> later = pages<UNIT>(t - 3 * WAVES);   // behind the LDS reads: scalar loads share their counter
             if constexpr (BF) weigh(vb8, s, t, now); else weigh(vf, s, t, now);
             if (!more) return;
             t -= WAVES; stage ^= STAGE;
@@ -247,20 +272,16 @@ struct Walk {
     }
 
     // softmax weights of the lane's E rows and their share of o
-    template <typename V>
-    __device__ __forceinline__ void weigh(V (&v)[4], const f32x4 (&s)[E / 4], int t, const Pages<T>& pg) {
+    template <typename V, int UNIT>
+    __device__ __forceinline__ void weigh(V (&v)[4], const f32x4 (&s)[E / 4], int t, const Pages<T, UNIT>& pg) {
         const int row0 = t * TILE<T> + g * E;
         const bool unset = ref == -__builtin_inff();
         const float base = __builtin_fmaf(slope2, (float)(row0 - (n - 1)), unset ? 0.f : -ref);
         float p[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) p[e] = __builtin_fmaf(c1, s[e >> 2][e & 3], base);
-        bool whole = t * TILE<T> + TILE<T> <= n;
-#pragma unroll
-        for (int c = 0; c < TILE<T> / 8; ++c) whole = whole && pg.ok[c];
-        if (!whole) {   // rows behind the length or on no page: no weight, and no bit of theirs in the product
-            bool ok;
-            if constexpr (BF) ok = g == 0 ? pg.ok[0] : g == 1 ? pg.ok[1] : g == 2 ? pg.ok[2] : pg.ok[3]; else ok = g < 2 ? pg.ok[0] : pg.ok[1];
+        if (t * TILE<T> + TILE<T> > n || pg.bad) {   // rows behind the length or on no page: no weight, and no bit of theirs in the product
+            const bool ok = !(pg.bad >> (g * E / UNIT) & 1);
 #pragma unroll
             for (int e = 0; e < E; ++e) p[e] = ok && row0 + e < n ? p[e] : -__builtin_inff();
             if constexpr (BF) {
@@ -411,7 +432,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(PagedAttnArgs
     const int kh = hp / a.passes, first = (hp - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
     Walk<T, WAVES> wk(a, lane, smem[w]);
     wk.begin(r, n, kh, head0, heads);
-    if (once) wk.template run<true>(t1 - 1 - w, t0); else wk.template run<false>(t1 - 1 - w, t0);
+    if (a.shift == 3) { if (once) wk.template run<8, true>(t1 - 1 - w, t0); else wk.template run<8, false>(t1 - 1 - w, t0); }
+    else { if (once) wk.template run<16, true>(t1 - 1 - w, t0); else wk.template run<16, false>(t1 - 1 - w, t0); }
     wk.leave();
     __syncthreads();
     const int d = (tid & 15) * 4;   // 16 threads a head, 4 dimensions each
