@@ -19,8 +19,8 @@
 //  * A wave instruction takes its SIMD four clocks, so what is the same for a whole tile or walk is kept off the vector unit: page ids, their
 //    checks and the addresses are scalar; the bias inside a tile is the C operand of the score product; the running maximum is compared lane by
 //    lane and reduced over lanes only when it moves by more than RISE; the sum of the probabilities is one more row of the value product.
-// MI355X, device time: 256 requests x 8 key heads, lengths 1 .. 4096, bf16 (1.07 GB): 177 us = 6.1 TB/s; 128 x 2 key heads, 1 .. 8192 (269 MB):
-// 58 us = 4.6 TB/s; 64 multi-query, 0 .. 2048 (17 MB): 11.3 us; one of 4096 rows (1 MB): 8.4 us in two launches, one of 256: 4.5 us in one.
+// MI355X, device time: 256 requests x 8 key heads, lengths 1 .. 4096, bf16 (1.07 GB): 176 us = 6.1 TB/s; 128 x 2 key heads, 1 .. 8192 (269 MB):
+// 56 us = 4.8 TB/s; 64 multi-query, 0 .. 2048 (17 MB): 10.3 us; one of 4096 rows (1 MB): 8.2 us in two launches, one of 256: 4.2 us in one.
 #include "common.h"
 #include "paged_index.h"
 
@@ -36,7 +36,7 @@ constexpr float RISE = 8.f;         // log2: probabilities up to 2^8 of the refe
 constexpr int MIN_TILES = 4;        // least tiles of a part (a tile per wave; 2: the same, 8: 1 x 4096 rows 8.9 -> 8.2 us the other way)
 constexpr int TARGET = 512;         // parts the batch is cut into, beside one per segment (1024: the same within 2 %)
 constexpr int MAX_TILES = 64;       // most tiles of a part where the batch is larger (32: 256 x 4096 rows 182 -> 196 us, 128: 186)
-constexpr int MAX_PARTS = 128;      // parts of a segment (one of 131072 rows, 256: 18.9 us, 128: 17.2, 64: 20.8)
+constexpr int MAX_PARTS = 128;      // parts of a segment (one of 131072 rows, 256: 18.9 us, 128: 17.2, 64: 20.8 when a tile cost a tenth more)
 
 template <typename T> constexpr int TILE = 64 / (int)sizeof(T);    // rows of a tile: 32 (bf16), 16 (fp32)
 
@@ -528,16 +528,16 @@ Split split_of(int R, int h, int kvh, int W, int shift, int esize) {
     const int group = h / kvh;
     s.passes = (group + HEADS - 1) / HEADS; s.rows = group < HEADS ? group : HEADS;
     const long segments = (long)R * kvh * s.passes, cap = (long)W << shift, bytes = cap * HEAD * 2 * esize, tiles = (bytes + STAGE - 1) / STAGE;
-    // Whole segments, one launch instead of two: a lone workgroup of 8 waves reads 78 GB/s (fp32, bound by its matrix instructions: 52), the machine
+    // Whole segments, one launch instead of two: a lone workgroup of 8 waves reads 105 GB/s (fp32, bound by its matrix instructions: 56), the machine
     // about 5 TB/s, the second launch costs some 6 us of device and host time, so with tables filled by half
     //   bytes / rate  <=  segments * bytes / 2 / 5 TB/s + 6 us,
-    // and never where one full table among short ones would take more than 14 us by itself (1 MiB: 4096 rows of a bf16 key head).
-    // Measured, whole / cut: 64 x 2048 rows 11.3 / 13.7 us, 1 x 4096 16.7 / 8.4, 16 x 512 5.4 / 8.6, 39 segments of 1001 fp32 rows 14.2 / 10.7,
-    // 2048 segments of up to 4096 rows 177 / 184.
-    const long rate = esize == 2 ? 78 : 52;   // bytes per ns
+    // and never where one full table among short ones would take long by itself (1 MiB: 10 us for 4096 rows of a bf16 key head, 19 for 2048 of fp32).
+    // Measured, whole / cut: 64 x 2048 rows 10.3 / 13.5 us, 1 x 4096 13.6 / 8.2, 16 x 512 5.1 / 8.2, 39 segments of 1001 fp32 rows 14.5 / 10.7,
+    // 2048 segments of up to 4096 rows 176 / 184.
+    const long rate = esize == 2 ? 105 : 56;   // bytes per ns
     const bool whole = bytes <= (1L << 20) && bytes * (10000 - rate * segments) <= 6000 * rate * 10000;
     // waves: 8 for long tables or few segments; many short segments leave most of 8 waves without a tile (2048 segments of up to 500 rows:
-    // 2 waves 27 us, 4: 30, 8: 40; 512 of up to 300 fp32 rows: 16.6, 13.8, 15.7; 2048 of up to 4096: 198, 182, 177)
+    // 2 waves 26.5 us, 4: 27.8, 8: 38.5; 512 of up to 1500: 23.0, 21.3, 22.3; 2048 of up to 4096: 193, 180, 176)
     s.waves = !whole ? 0 : segments > 256 ? (tiles >= 64 ? 8 : tiles > 16 ? 4 : 2) : tiles > 8 ? 8 : 4;
     s.once = segments * bytes >= 2 * ONCE;   // tables filled by half
     // the longest part: MAX_TILES, or what keeps the grid -- all tables full -- to 8192 parts
