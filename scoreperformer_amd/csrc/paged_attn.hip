@@ -36,6 +36,7 @@ constexpr float RISE = 8.f;         // log2: probabilities up to 2^8 of the refe
 constexpr int MIN_TILES = 4;        // least tiles of a part (a tile per wave; 2: the same, 8: 1 x 4096 rows 8.9 -> 8.2 us the other way)
 constexpr int TARGET = 512;         // parts the batch is cut into, beside one per segment (1024: the same within 2 %)
 constexpr int MAX_TILES = 64;       // most tiles of a part where the batch is larger (32: 256 x 4096 rows 182 -> 196 us, 128: 186)
+constexpr unsigned GRID = 1024;     // workgroups of a cut batch (twice what is resident at once)
 constexpr int MAX_PARTS = 128;      // parts of a segment (one of 131072 rows, 256: 18.9 us, 128: 17.2, 64: 20.8 when a tile cost a tenth more)
 
 template <typename T> constexpr int TILE = 64 / (int)sizeof(T);    // rows of a tile: 32 (bf16), 16 (fp32)
@@ -47,7 +48,8 @@ struct PagedAttnArgs {
     int rows;                  // heads of a partial result: min(group, 16)
     int max_tiles;             // most tiles of a part
     int once;                  // whole segments: do not keep the rows in the caches (cut ones: decided on the device)
-    float* part; float* ml; int4* hdr;   // [G][rows][64], [G][rows][2], [G] {request, key head and pass, parts (its first part only), 0}
+    int units;                 // room for this many parts
+    float* part; float* ml; int4* hdr;   // [units][rows][64], [units][rows][2], {parts of the batch}, [units] {request, key head and pass, parts (its first part only), 0}
 };
 
 // reductions over the four lanes of a head (l, l ^ 16, l ^ 32, l ^ 48): the swapped halves of two copies, no LDS crossbar
@@ -383,52 +385,10 @@ __device__ __forceinline__ int parts_of(int tiles, int most) { return max(1, min
 constexpr long ONCE = 64L << 20;   // bytes of rows from which they are not kept in the caches (Infinity Cache: 256 MiB; a step walks every layer's cache
                                    // before it is back at this one).  1.07 GB: 195 -> 177 us; 17 MB, three pools in turn: 11.4 -> 13.3 us, hence the bound
 
-// One workgroup, one part of one segment.  DIRECT: the whole of it.  Otherwise every wave adds up the batch's tiles for itself (a lane: every 64th
-// stretch of requests; no barrier, no LDS), takes a TARGET-th of them as the longest part, and finds the request whose parts workgroup number wg is
-// among.
-template <typename T, bool DIRECT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(PagedAttnArgs a) {
-    __shared__ __attribute__((aligned(1024))) char smem[WAVES][2 * STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), H = a.kvh * a.passes;
-    const int wg = blockIdx.x;
-    int r, n, hp, part = 0, parts = 1;
-    bool once = a.once;
-    if constexpr (DIRECT) {
-        r = wg / H; hp = wg - r * H;
-        n = rows_at(a, r);
-    } else {
-        const int per = (a.R + 63) / 64, q0 = min(a.R, lane * per), q1 = min(a.R, q0 + per);   // this lane's requests
-        const int first = q0 < q1 ? rows_at(a, q0) : 0;
-        long mine = tiles_in<T>(first);
-        for (int q = q0 + 1; q < q1; ++q) mine += tiles_in<T>(rows_at(a, q));
-        // in two halves of 32 bits: table capacities pass 2^32 tiles before memory does
-        const long total = H * (((long)__builtin_amdgcn_readlane(wave_scan((int)(mine >> 16)), 63) << 16) +
-                                (uint32_t)__builtin_amdgcn_readlane(wave_scan((int)(mine & 0xffff)), 63));
-        const int most = (int)min(max((long)MIN_TILES, (total + TARGET - 1) / TARGET), (long)a.max_tiles);
-        once = total * STAGE >= ONCE;
-        int units = q0 < q1 ? H * parts_of(tiles_in<T>(first), most) : 0;
-        for (int q = q0 + 1; q < q1; ++q) units += H * parts_of(tiles_in<T>(rows_at(a, q)), most);
-        const int incl = wave_scan(units);
-        const unsigned long long behind = __ballot(incl > wg);
-        if (!behind) {
-            if (tid == 0) a.hdr[wg] = int4{0, 0, 0, 0};
-            return;
-        }
-        const int at = __builtin_ctzll(behind);
-        int off = wg - __builtin_amdgcn_readlane(incl - units, at);
-        r = at * per;
-        n = __builtin_amdgcn_readlane(first, at);
-        for (;;) {
-            parts = parts_of(tiles_in<T>(n), most);
-            if (off < H * parts || r + 1 >= a.R) break;
-            off -= H * parts;
-            n = rows_at(a, ++r);   // (a lane's later requests: more than 64 in the batch)
-        }
-        // (the bounds hold by themselves unless the lengths change while this runs; then the result is lost, but no access goes astray)
-        hp = min(off / parts, H - 1); part = min(off - hp * parts, parts - 1);
-    }
-    const int tiles = tiles_in<T>(n);
-    const int t0 = DIRECT ? 0 : (int)((long)tiles * part / parts), t1 = DIRECT ? tiles : (int)((long)tiles * (part + 1) / parts);
+// One part of one segment: the walks of the workgroup's waves, and their results put together -- into the output, or (slot >= 0) into a partial result.
+template <typename T, int WAVES>
+__device__ __forceinline__ void do_part(const PagedAttnArgs& a, char (*smem)[2 * STAGE], int tid, int r, int n, int hp, int t0, int t1, bool once, long slot) {
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kh = hp / a.passes, first = (hp - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
     Walk<T, WAVES> wk(a, lane, smem[w]);
     wk.begin(r, n, kh, head0, heads);
@@ -450,18 +410,61 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_kernel(PagedAttnArgs
 #pragma unroll
             for (int e = 0; e < 4; ++e) O[e] += c * ov[e];
         }
-        if (DIRECT || parts == 1) {
+        if (slot < 0) {
             const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
             for (int e = 0; e < 4; ++e) O[e] = L == 0.f ? 0.f : O[e] * inv;
             store4((T*)a.o + r * a.o_rs + (long)(head0 + hd) * a.o_hs + d, O);
         } else {
-            const long slot = (long)wg * a.rows + hd;
-            *reinterpret_cast<f32x4*>(a.part + slot * HEAD + d) = f32x4{O[0], O[1], O[2], O[3]};
-            if (d == 0) { a.ml[2 * slot] = M; a.ml[2 * slot + 1] = L; }
+            const long at = slot * a.rows + hd;
+            *reinterpret_cast<f32x4*>(a.part + at * HEAD + d) = f32x4{O[0], O[1], O[2], O[3]};
+            if (d == 0) { a.ml[2 * at] = M; a.ml[2 * at + 1] = L; }
         }
     }
-    if (!DIRECT && tid == 0) a.hdr[wg] = int4{r, hp, part == 0 && parts > 1 ? parts : 0, 0};
+}
+
+// A workgroup takes a whole segment.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_whole_kernel(PagedAttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[WAVES][2 * STAGE];
+    const int H = a.kvh * a.passes, wg = blockIdx.x, r = wg / H, n = rows_at(a, r);
+    do_part<T, WAVES>(a, smem, threadIdx.x, r, n, wg - r * H, 0, tiles_in<T>(n), a.once, -1);
+}
+
+// Segments cut into parts.  Every wave adds up the batch's tiles for itself (a lane: every 64th stretch of requests; no barrier, no LDS) and takes a
+// TARGET-th of them as the longest part; the parts of all segments stand in one line, of which workgroup g takes number g, g + G, ...
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_cut_kernel(PagedAttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[WAVES][2 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, H = a.kvh * a.passes;
+    const int per = (a.R + 63) / 64, q0 = min(a.R, lane * per), q1 = min(a.R, q0 + per);   // this lane's requests
+    const int first = q0 < q1 ? rows_at(a, q0) : 0;
+    long mine = tiles_in<T>(first);
+    for (int q = q0 + 1; q < q1; ++q) mine += tiles_in<T>(rows_at(a, q));
+    // in two halves of 32 bits: table capacities pass 2^32 tiles before memory does
+    const long total = H * (((long)__builtin_amdgcn_readlane(wave_scan((int)(mine >> 16)), 63) << 16) +
+                            (uint32_t)__builtin_amdgcn_readlane(wave_scan((int)(mine & 0xffff)), 63));
+    const int most = (int)min(max((long)MIN_TILES, (total + TARGET - 1) / TARGET), (long)a.max_tiles);
+    const bool once = total * STAGE >= ONCE;
+    int units = q0 < q1 ? H * parts_of(tiles_in<T>(first), most) : 0;
+    for (int q = q0 + 1; q < q1; ++q) units += H * parts_of(tiles_in<T>(rows_at(a, q)), most);
+    const int incl = wave_scan(units), all = min(__builtin_amdgcn_readlane(incl, 63), a.units);
+    if (blockIdx.x == 0 && tid == 0) a.hdr[0] = int4{all, 0, 0, 0};
+    for (int u = blockIdx.x; u < all; u += gridDim.x) {
+        const int at = __builtin_ctzll(__ballot(incl > u));
+        int off = u - __builtin_amdgcn_readlane(incl - units, at), r = at * per, n = __builtin_amdgcn_readlane(first, at), parts;
+        for (;;) {
+            parts = parts_of(tiles_in<T>(n), most);
+            if (off < H * parts || r + 1 >= a.R) break;
+            off -= H * parts;
+            n = rows_at(a, ++r);   // (a lane's later requests: more than 64 in the batch)
+        }
+        // (the bounds hold by themselves unless the lengths change while this runs; then the result is lost, but no access goes astray)
+        const int hp = min(off / parts, H - 1), part = min(off - hp * parts, parts - 1), tiles = tiles_in<T>(n);
+        do_part<T, WAVES>(a, smem, tid, r, n, hp, (int)((long)tiles * part / parts), (int)((long)tiles * (part + 1) / parts), once, parts > 1 ? u : -1);
+        if (tid == 0) a.hdr[1 + u] = int4{r, hp, part == 0 && parts > 1 ? parts : 0, 0};
+        __syncthreads();   // the tiles of the next part go where this one's results were
+    }
 }
 
 // Joins the parts of a segment that was cut: slots g .. g + parts - 1, in a fixed order.  JOIN_HEADS heads a block; 16 lanes (4 dimensions each) take
@@ -470,59 +473,63 @@ constexpr int JOIN_HEADS = 2, JOIN_SUBS = 16 / JOIN_HEADS;
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     __shared__ float s_o[16][LDO], s_m[16], s_l[16];
-    const long wg = blockIdx.x;
-    const int4 cut = a.hdr[wg];
-    if (cut.z == 0) return;
-    const int kh = cut.y / a.passes, first = (cut.y - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
-    const int grp = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, sub = grp % JOIN_SUBS, hd = blockIdx.y * JOIN_HEADS + grp / JOIN_SUBS;
-    float M = -__builtin_inff(), L = 0.f;
-    f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (hd < heads) {
-        const float* ml = a.ml + 2 * (wg * a.rows + hd);
-        const float* po = a.part + (wg * a.rows + hd) * HEAD + d;
-        constexpr int U = 8;
-        for (int p = sub; p < cut.z; p += JOIN_SUBS * U) {
-            float m[U], l[U];
-            f32x4 o[U];
+    const int all = min(a.hdr[0].x, a.units), grp = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, sub = grp % JOIN_SUBS;
+    const int hd = blockIdx.y * JOIN_HEADS + grp / JOIN_SUBS;
+    for (int g = blockIdx.x; g < all; g += gridDim.x) {
+        const int4 cut = a.hdr[1 + g];
+        if (cut.z == 0) continue;
+        const int parts = min(cut.z, all - g);
+        const int kh = cut.y / a.passes, first = (cut.y - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
+        float M = -__builtin_inff(), L = 0.f;
+        f32x4 O = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (hd < heads) {
+            const float* ml = a.ml + 2 * ((long)g * a.rows + hd);
+            const float* po = a.part + ((long)g * a.rows + hd) * HEAD + d;
+            constexpr int U = 8;
+            for (int p = sub; p < parts; p += JOIN_SUBS * U) {
+                float m[U], l[U];
+                f32x4 o[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const long at = (long)min(p + u * JOIN_SUBS, cut.z - 1) * a.rows;
-                m[u] = ml[2 * at]; l[u] = ml[2 * at + 1];
-                o[u] = *reinterpret_cast<const f32x4*>(po + at * HEAD);
-            }
+                for (int u = 0; u < U; ++u) {
+                    const long at = (long)min(p + u * JOIN_SUBS, parts - 1) * a.rows;
+                    m[u] = ml[2 * at]; l[u] = ml[2 * at + 1];
+                    o[u] = *reinterpret_cast<const f32x4*>(po + at * HEAD);
+                }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (p + u * JOIN_SUBS >= cut.z) { m[u] = -__builtin_inff(); l[u] = 0.f; o[u] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-                const float mn = fmaxf(M, m[u]), c = M == mn ? 1.f : __builtin_amdgcn_exp2f(M - mn), b = under(m[u], mn);
-                L = L * c + l[u] * b; M = mn;
+                for (int u = 0; u < U; ++u) {
+                    if (p + u * JOIN_SUBS >= parts) { m[u] = -__builtin_inff(); l[u] = 0.f; o[u] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+                    const float mn = fmaxf(M, m[u]), c = M == mn ? 1.f : __builtin_amdgcn_exp2f(M - mn), b = under(m[u], mn);
+                    L = L * c + l[u] * b; M = mn;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) O[e] = O[e] * c + o[u][e] * b;
+                    for (int e = 0; e < 4; ++e) O[e] = O[e] * c + o[u][e] * b;
+                }
             }
         }
-    }
-    *reinterpret_cast<f32x4*>(&s_o[grp][d]) = O;
-    if (d == 0) { s_m[grp] = M; s_l[grp] = L; }
-    __syncthreads();
-    if (sub == 0 && hd < heads) {
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        M = -__builtin_inff(); L = 0.f;
+        __syncthreads();   // (the previous one has been read)
+        *reinterpret_cast<f32x4*>(&s_o[grp][d]) = O;
+        if (d == 0) { s_m[grp] = M; s_l[grp] = L; }
+        __syncthreads();
+        if (sub == 0 && hd < heads) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            M = -__builtin_inff(); L = 0.f;
 #pragma unroll
-        for (int u = 0; u < JOIN_SUBS; ++u) M = fmaxf(M, s_m[grp + u]);
+            for (int u = 0; u < JOIN_SUBS; ++u) M = fmaxf(M, s_m[grp + u]);
 #pragma unroll
-        for (int u = 0; u < JOIN_SUBS; ++u) {
-            const float c = under(s_m[grp + u], M);
-            L += c * s_l[grp + u];
+            for (int u = 0; u < JOIN_SUBS; ++u) {
+                const float c = under(s_m[grp + u], M);
+                L += c * s_l[grp + u];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += c * s_o[grp + u][d + e];
+                for (int e = 0; e < 4; ++e) v[e] += c * s_o[grp + u][d + e];
+            }
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = L == 0.f ? 0.f : v[e] * inv;
+            store4((T*)a.o + cut.x * a.o_rs + (long)(head0 + hd) * a.o_hs + d, v);
         }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = L == 0.f ? 0.f : v[e] * inv;
-        store4((T*)a.o + cut.x * a.o_rs + (long)(head0 + hd) * a.o_hs + d, v);
     }
 }
 
-struct Split { long grid; int waves; int passes, rows, max_tiles, once; };   // waves: of a workgroup that takes a whole segment; 0: cut
+struct Split { long units; int waves; int passes, rows, max_tiles, once; };   // waves: of a workgroup that takes a whole segment; 0: cut
 Split split_of(int R, int h, int kvh, int W, int shift, int esize) {
     Split s;
     const int group = h / kvh;
@@ -540,14 +547,14 @@ Split split_of(int R, int h, int kvh, int W, int shift, int esize) {
     // 2 waves 26.5 us, 4: 27.8, 8: 38.5; 512 of up to 1500: 23.0, 21.3, 22.3; 2048 of up to 4096: 193, 180, 176)
     s.waves = !whole ? 0 : segments > 256 ? (tiles >= 64 ? 8 : tiles > 16 ? 4 : 2) : tiles > 8 ? 8 : 4;
     s.once = segments * bytes >= 2 * ONCE;   // tables filled by half
-    // the longest part: MAX_TILES, or what keeps the grid -- all tables full -- to 8192 parts
+    // the longest part: MAX_TILES, or what keeps the workspace -- all tables full -- to 8192 parts
     const long full = segments * tiles, most = (full + 8191) / 8192;
     s.max_tiles = (int)(most < MAX_TILES ? MAX_TILES : most);
     // parts on the device: at most tiles / most + 1 for each segment, with most >= MIN_TILES and most >= min(max_tiles, all tiles / TARGET)
     long units = full / s.max_tiles;
     units = (units < TARGET ? TARGET : units) + segments;
     const long finest = segments * ((tiles + MIN_TILES - 1) / MIN_TILES);
-    s.grid = whole ? segments : units < finest ? units : finest;
+    s.units = whole ? segments : units < finest ? units : finest;
     return s;
 }
 
@@ -556,21 +563,22 @@ int page_shift(int page) {
     return -1;
 }
 
-size_t scratch_of(const Split& s) { return s.waves ? 0 : (size_t)s.grid * ((size_t)s.rows * (HEAD + 2) * sizeof(float) + sizeof(int4)); }
+size_t scratch_of(const Split& s) { return s.waves ? 0 : (size_t)s.units * ((size_t)s.rows * (HEAD + 2) * sizeof(float) + sizeof(int4)) + sizeof(int4); }
 
-template <typename T, bool DIRECT, int WAVES>
-void launch(const PagedAttnArgs& a, long grid, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_attn_kernel<T, DIRECT, WAVES>), dim3((unsigned)grid), dim3(64 * WAVES), 0, stream, a);
+template <typename T, int WAVES>
+void launch_whole(const PagedAttnArgs& a, long segments, hipStream_t stream) {
+    hipLaunchKernelGGL((paged_attn_whole_kernel<T, WAVES>), dim3((unsigned)segments), dim3(64 * WAVES), 0, stream, a);
 }
 template <typename T>
-int launch_all(const PagedAttnArgs& a, const Split& s, hipStream_t stream) {
-    if (s.waves == 8) launch<T, true, 8>(a, s.grid, stream);
-    else if (s.waves == 4) launch<T, true, 4>(a, s.grid, stream);
-    else if (s.waves == 2) launch<T, true, 2>(a, s.grid, stream);
+int launch(const PagedAttnArgs& a, const Split& s, hipStream_t stream) {
+    if (s.waves == 8) launch_whole<T, 8>(a, s.units, stream);
+    else if (s.waves == 4) launch_whole<T, 4>(a, s.units, stream);
+    else if (s.waves == 2) launch_whole<T, 2>(a, s.units, stream);
     else {
-        launch<T, false, 4>(a, s.grid, stream);
+        const unsigned grid = s.units < GRID ? (unsigned)s.units : GRID;
+        hipLaunchKernelGGL((paged_attn_cut_kernel<T, 4>), dim3(grid), dim3(256), 0, stream, a);
         SPN_LAUNCH_CHECK();
-        hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)s.grid, cdiv(a.rows, JOIN_HEADS)), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(paged_join_kernel<T>, dim3(grid, cdiv(a.rows, JOIN_HEADS)), dim3(256), 0, stream, a);
     }
     SPN_LAUNCH_CHECK();
     return SPN_OK;
@@ -599,7 +607,7 @@ extern "C" int spn_paged_attn(const void* q, long q_rs, long q_hs, const void* k
     SPN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                 "spn_paged_attn: the workspace is too small or not 16-byte aligned (spn_paged_attn_workspace_bytes)");
     PagedAttnArgs a{q, q_rs, q_hs, k_pages, v_pages, block_table, bt_ld, lens, slopes, o, o_rs, o_hs, R, h, kvh, W, num_pages, shift, scale,
-                    h / kvh, s.passes, s.rows, s.max_tiles, s.once, nullptr, nullptr, nullptr};
-    if (need) { a.hdr = (int4*)workspace; a.part = (float*)(a.hdr + s.grid); a.ml = a.part + s.grid * s.rows * HEAD; }
-    return dtype == 1 ? launch_all<bf16_t>(a, s, stream) : launch_all<float>(a, s, stream);
+                    h / kvh, s.passes, s.rows, s.max_tiles, s.once, (int)s.units, nullptr, nullptr, nullptr};
+    if (need) { a.hdr = (int4*)workspace; a.part = (float*)(a.hdr + 1 + s.units); a.ml = a.part + s.units * s.rows * HEAD; }
+    return dtype == 1 ? launch<bf16_t>(a, s, stream) : launch<float>(a, s, stream);
 }
