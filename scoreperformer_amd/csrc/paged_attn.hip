@@ -5,8 +5,8 @@
 // Every cached row is read once: 2 * kvh * 64 * sizeof(T) bytes per row against 4 * h * 64 flop -- bound by HBM for every head layout, as long
 // as enough loads are in flight, and below some 10 MB by the chain length -> page id -> rows -> softmax -> sum of one workgroup (4 us).
 //  * A segment (request, key head, 16 query heads of it) is one workgroup's, or is cut into parts of at most a 512th of the batch's rows: the
-//    device counts the batch itself, so one long cache among short ones, or a table far wider than the lengths, costs nothing and no length is
-//    known to the host.  Parts leave (max, sum, unnormalised o) in the workspace; a second, small launch joins them in a fixed order.
+//    device counts the batch itself, so no length is known to the host and one long cache among short ones does not set the time; a fixed grid
+//    walks the parts, so a table far wider than the lengths costs the second launch and little else.  Parts leave (max, sum, unnormalised o) in the workspace; a second, small launch joins them in a fixed order.
 //  * Rows travel HBM -> LDS by DMA in whole 1 KiB pieces, 16 bytes a lane, consecutive lanes on consecutive bytes.  (The layouts the matrix
 //    instructions want, loaded straight into registers -- a lane per row, 64 of a row's 128 bytes at a time -- hold one CU to 37 GB/s where
 //    whole pieces reach 105: the first-level cache serves four lanes of one line per clock.)  Two tiles of 8 KiB per wave, private to it: no barrier.
@@ -19,8 +19,8 @@
 //  * A wave instruction takes its SIMD four clocks, so what is the same for a whole tile or walk is kept off the vector unit: page ids, their
 //    checks and the addresses are scalar; the bias inside a tile is the C operand of the score product; the running maximum is compared lane by
 //    lane and reduced over lanes only when it moves by more than RISE; the sum of the probabilities is one more row of the value product.
-// MI355X, device time: 256 requests x 8 key heads, lengths 1 .. 4096, bf16 (1.07 GB): 176 us = 6.1 TB/s; 128 x 2 key heads, 1 .. 8192 (269 MB):
-// 56 us = 4.8 TB/s; 64 multi-query, 0 .. 2048 (17 MB): 10.3 us; one of 4096 rows (1 MB): 8.2 us in two launches, one of 256: 4.2 us in one.
+// MI355X, device time: 256 requests x 8 key heads, lengths 1 .. 4096, bf16 (1.07 GB): 180 us = 6.0 TB/s; 128 x 2 key heads, 1 .. 8192 (269 MB):
+// 57 us = 4.7 TB/s; 64 multi-query, 0 .. 2048 (17 MB): 10.4 us; one of 4096 rows (1 MB): 8.3 us in two launches, one of 256: 4.2 us in one.
 #include "common.h"
 #include "paged_index.h"
 
@@ -36,7 +36,8 @@ constexpr float RISE = 8.f;         // log2: probabilities up to 2^8 of the refe
 constexpr int MIN_TILES = 4;        // least tiles of a part (a tile per wave; 2: the same, 8: 1 x 4096 rows 8.9 -> 8.2 us the other way)
 constexpr int TARGET = 512;         // parts the batch is cut into, beside one per segment (1024: the same within 2 %)
 constexpr int MAX_TILES = 64;       // most tiles of a part where the batch is larger (32: 256 x 4096 rows 182 -> 196 us, 128: 186)
-constexpr unsigned GRID = 1024;     // workgroups of a cut batch (twice what is resident at once)
+constexpr int RESIDENT = 512;       // workgroups of 4 waves that run at once: two on a compute unit, by their LDS
+constexpr unsigned GRID = 2 * RESIDENT;   // workgroups of a cut batch
 constexpr int MAX_PARTS = 128;      // parts of a segment (one of 131072 rows, 256: 18.9 us, 128: 17.2, 64: 20.8 when a tile cost a tenth more)
 
 template <typename T> constexpr int TILE = 64 / (int)sizeof(T);    // rows of a tile: 32 (bf16), 16 (fp32)
@@ -385,17 +386,21 @@ __device__ __forceinline__ int parts_of(int tiles, int most) { return max(1, min
 constexpr long ONCE = 64L << 20;   // bytes of rows from which they are not kept in the caches (Infinity Cache: 256 MiB; a step walks every layer's cache
                                    // before it is back at this one).  1.07 GB: 195 -> 177 us; 17 MB, three pools in turn: 11.4 -> 13.3 us, hence the bound
 
-// One part of one segment: the walks of the workgroup's waves, and their results put together -- into the output, or (slot >= 0) into a partial result.
+// tiles [t0, t1) of segment hp (key head and 16-head pass) of request r, which holds n rows; parts: into how many the segment is cut
+struct Part { int r, n, hp, t0, t1, part, parts; };
+
+// One part of one segment by WAVES waves (threads tid, LDS smem): their walks, and their results put together -- into the output, or (slot >= 0) into
+// a partial result.
 template <typename T, int WAVES>
-__device__ __forceinline__ void do_part(const PagedAttnArgs& a, char (*smem)[2 * STAGE], int tid, int r, int n, int hp, int t0, int t1, bool once, long slot) {
-    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kh = hp / a.passes, first = (hp - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
+__device__ __forceinline__ void do_part(const PagedAttnArgs& a, char (*smem)[2 * STAGE], int tid, const Part& p, bool once, long slot) {
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = p.r;
+    const int kh = p.hp / a.passes, first = (p.hp - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
     Walk<T, WAVES> wk(a, lane, smem[w]);
-    wk.begin(r, n, kh, head0, heads);
-    if (a.shift == 3) { if (once) wk.template run<8, true>(t1 - 1 - w, t0); else wk.template run<8, false>(t1 - 1 - w, t0); }
-    else { if (once) wk.template run<16, true>(t1 - 1 - w, t0); else wk.template run<16, false>(t1 - 1 - w, t0); }
+    wk.begin(r, p.n, kh, head0, heads);
+    if (a.shift == 3) { if (once) wk.template run<8, true>(p.t1 - 1 - w, p.t0); else wk.template run<8, false>(p.t1 - 1 - w, p.t0); }
+    else { if (once) wk.template run<16, true>(p.t1 - 1 - w, p.t0); else wk.template run<16, false>(p.t1 - 1 - w, p.t0); }
     wk.leave();
-    __syncthreads();
+    if constexpr (WAVES == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); else __syncthreads();
     const int d = (tid & 15) * 4;   // 16 threads a head, 4 dimensions each
     for (int hd = tid >> 4; hd < heads; hd += 4 * WAVES) {
         float M = -__builtin_inff(), L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
@@ -423,19 +428,44 @@ __device__ __forceinline__ void do_part(const PagedAttnArgs& a, char (*smem)[2 *
     }
 }
 
+// Four parts by four waves: a wave each where all are short, otherwise one after the other by all four.  A short part costs its latency, not its
+// bytes: 8000 segments of up to 100 rows 104 -> 55 us.
+constexpr int SHORT = 24;   // tiles
+template <typename T, typename At, typename Done>
+__device__ __forceinline__ void do_four(const PagedAttnArgs& a, char (*smem)[2 * STAGE], int tid, int u, int all, bool once, const At& at, const Done& done) {
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int longest = 0;
+    for (int k = 0; k < 4 && u + k < all; ++k) { const Part p = at(u + k); longest = max(longest, p.t1 - p.t0); }
+    if (longest <= SHORT) {
+        if (u + w < all) {
+            const Part p = at(u + w);
+            do_part<T, 1>(a, smem + w, tid & 63, p, once, p.parts > 1 ? u + w : -1);
+            if ((tid & 63) == 0) done(u + w, p);
+        }
+    } else {
+        for (int k = 0; k < 4 && u + k < all; ++k) {
+            if (k) __syncthreads();
+            const Part p = at(u + k);
+            do_part<T, 4>(a, smem, tid, p, once, p.parts > 1 ? u + k : -1);
+            if (tid == 0) done(u + k, p);
+        }
+    }
+}
+
 // A workgroup takes a whole segment.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_whole_kernel(PagedAttnArgs a) {
     __shared__ __attribute__((aligned(1024))) char smem[WAVES][2 * STAGE];
-    const int H = a.kvh * a.passes, wg = blockIdx.x, r = wg / H, n = rows_at(a, r);
-    do_part<T, WAVES>(a, smem, threadIdx.x, r, n, wg - r * H, 0, tiles_in<T>(n), a.once, -1);
+    const int H = a.kvh * a.passes, r = blockIdx.x / H, n = rows_at(a, r);
+    do_part<T, WAVES>(a, smem, threadIdx.x, Part{r, n, (int)blockIdx.x - r * H, 0, tiles_in<T>(n), 0, 1}, a.once, -1);
 }
 
 // Segments cut into parts.  Every wave adds up the batch's tiles for itself (a lane: every 64th stretch of requests; no barrier, no LDS) and takes a
-// TARGET-th of them as the longest part; the parts of all segments stand in one line, of which workgroup g takes number g, g + G, ...
-template <typename T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_cut_kernel(PagedAttnArgs a) {
-    __shared__ __attribute__((aligned(1024))) char smem[WAVES][2 * STAGE];
+// TARGET-th of them as the longest part; the parts of all segments stand in one line, of which workgroup g takes number g, g + G, ...  (four at a
+// time where there are enough of them).
+template <typename T>
+__global__ __launch_bounds__(256, 2) void paged_attn_cut_kernel(PagedAttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[4][2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, H = a.kvh * a.passes;
     const int per = (a.R + 63) / 64, q0 = min(a.R, lane * per), q1 = min(a.R, q0 + per);   // this lane's requests
     const int first = q0 < q1 ? rows_at(a, q0) : 0;
@@ -450,20 +480,45 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_cut_kernel(PagedAttn
     for (int q = q0 + 1; q < q1; ++q) units += H * parts_of(tiles_in<T>(rows_at(a, q)), most);
     const int incl = wave_scan(units), all = min(__builtin_amdgcn_readlane(incl, 63), a.units);
     if (blockIdx.x == 0 && tid == 0) a.hdr[0] = int4{all, 0, 0, 0};
-    for (int u = blockIdx.x; u < all; u += gridDim.x) {
-        const int at = __builtin_ctzll(__ballot(incl > u));
-        int off = u - __builtin_amdgcn_readlane(incl - units, at), r = at * per, n = __builtin_amdgcn_readlane(first, at), parts;
-        for (;;) {
-            parts = parts_of(tiles_in<T>(n), most);
-            if (off < H * parts || r + 1 >= a.R) break;
-            off -= H * parts;
-            n = rows_at(a, ++r);   // (a lane's later requests: more than 64 in the batch)
+    const auto at = [&](int u) {
+        Part p;
+        const int from = __builtin_ctzll(__ballot(incl > u));
+        int off = u - __builtin_amdgcn_readlane(incl - units, from);
+        p.r = from * per; p.n = __builtin_amdgcn_readlane(first, from);
+        // more than 64 requests: those of the lane that was found, 64 at a time, a lane each
+        for (int base = p.r; per > 1; base += 64) {
+            const int q = base + lane, mine = q < min((from + 1) * per, a.R) ? rows_at(a, q) : 0;
+            const int here = q < min((from + 1) * per, a.R) ? H * parts_of(tiles_in<T>(mine), most) : 0, to = wave_scan(here);
+            const unsigned long long found = __ballot(to > off);
+            const bool last = base + 64 >= min((from + 1) * per, a.R);
+            if (found || last) {
+                const int k = found ? __builtin_ctzll(found) : 0;
+                p.r = base + k; p.n = __builtin_amdgcn_readlane(mine, k);
+                off -= __builtin_amdgcn_readlane(to - here, k);
+                break;
+            }
+            off -= __builtin_amdgcn_readlane(to, 63);
         }
+        p.parts = parts_of(tiles_in<T>(p.n), most);
         // (the bounds hold by themselves unless the lengths change while this runs; then the result is lost, but no access goes astray)
-        const int hp = min(off / parts, H - 1), part = min(off - hp * parts, parts - 1), tiles = tiles_in<T>(n);
-        do_part<T, WAVES>(a, smem, tid, r, n, hp, (int)((long)tiles * part / parts), (int)((long)tiles * (part + 1) / parts), once, parts > 1 ? u : -1);
-        if (tid == 0) a.hdr[1 + u] = int4{r, hp, part == 0 && parts > 1 ? parts : 0, 0};
-        __syncthreads();   // the tiles of the next part go where this one's results were
+        p.hp = min(off / p.parts, H - 1); p.part = min(off - p.hp * p.parts, p.parts - 1);
+        const int tiles = tiles_in<T>(p.n);
+        p.t0 = (int)((long)tiles * p.part / p.parts); p.t1 = (int)((long)tiles * (p.part + 1) / p.parts);
+        return p;
+    };
+    const auto done = [&](int u, const Part& p) { a.hdr[1 + u] = int4{p.r, p.hp, p.part == 0 && p.parts > 1 ? p.parts : 0, 0}; };
+    if (all >= 4 * RESIDENT && total <= (long)all * (SHORT / 2)) {
+        for (int u = 4 * blockIdx.x; u < all; u += 4 * gridDim.x) {
+            do_four<T>(a, smem, tid, u, all, once, at, done);
+            __syncthreads();   // the tiles of the next parts go where these results were
+        }
+    } else {
+        for (int u = blockIdx.x; u < all; u += gridDim.x) {
+            const Part p = at(u);
+            do_part<T, 4>(a, smem, tid, p, once, p.parts > 1 ? u : -1);
+            if (tid == 0) done(u, p);
+            __syncthreads();
+        }
     }
 }
 
@@ -473,10 +528,11 @@ constexpr int JOIN_HEADS = 2, JOIN_SUBS = 16 / JOIN_HEADS;
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     __shared__ float s_o[16][LDO], s_m[16], s_l[16];
+    int4 cut = a.hdr[1 + blockIdx.x];   // (written or not: asked for together with the count)
     const int all = min(a.hdr[0].x, a.units), grp = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, sub = grp % JOIN_SUBS;
     const int hd = blockIdx.y * JOIN_HEADS + grp / JOIN_SUBS;
     for (int g = blockIdx.x; g < all; g += gridDim.x) {
-        const int4 cut = a.hdr[1 + g];
+        if (g != (int)blockIdx.x) cut = a.hdr[1 + g];
         if (cut.z == 0) continue;
         const int parts = min(cut.z, all - g);
         const int kh = cut.y / a.passes, first = (cut.y - kh * a.passes) * HEADS, heads = min(HEADS, a.group - first), head0 = kh * a.group + first;
@@ -543,9 +599,10 @@ Split split_of(int R, int h, int kvh, int W, int shift, int esize) {
     // 2048 segments of up to 4096 rows 176 / 184.
     const long rate = esize == 2 ? 105 : 56;   // bytes per ns
     const bool whole = bytes <= (1L << 20) && bytes * (10000 - rate * segments) <= 6000 * rate * 10000;
-    // waves: 8 for long tables or few segments; many short segments leave most of 8 waves without a tile (2048 segments of up to 500 rows:
-    // 2 waves 26.5 us, 4: 27.8, 8: 38.5; 512 of up to 1500: 23.0, 21.3, 22.3; 2048 of up to 4096: 193, 180, 176)
-    s.waves = !whole ? 0 : segments > 256 ? (tiles >= 64 ? 8 : tiles > 16 ? 4 : 2) : tiles > 8 ? 8 : 4;
+    // waves: 8 where the segments do not fill the machine.  Where they do, their lengths decide, which the host does not know: 8 waves serve long rows
+    // best (2048 segments of up to 4096 rows, 2 / 4 / 8 waves: 193, 180, 176 us), 2 waves short ones (8000 of up to 100: 30, 50, 89; 2048 of up to
+    // 500: 26, 28, 38; of up to 1000: 45, 43, 51), so the width of the tables is the hint and 8 is left out
+    s.waves = !whole ? 0 : segments >= 4 * RESIDENT ? (tiles > 64 ? 4 : 2) : segments > 256 ? 4 : tiles > 8 ? 8 : 4;
     s.once = segments * bytes >= 2 * ONCE;   // tables filled by half
     // the longest part: MAX_TILES, or what keeps the workspace -- all tables full -- to 8192 parts
     const long full = segments * tiles, most = (full + 8191) / 8192;
@@ -576,7 +633,7 @@ int launch(const PagedAttnArgs& a, const Split& s, hipStream_t stream) {
     else if (s.waves == 2) launch_whole<T, 2>(a, s.units, stream);
     else {
         const unsigned grid = s.units < GRID ? (unsigned)s.units : GRID;
-        hipLaunchKernelGGL((paged_attn_cut_kernel<T, 4>), dim3(grid), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(paged_attn_cut_kernel<T>, dim3(grid), dim3(256), 0, stream, a);
         SPN_LAUNCH_CHECK();
         hipLaunchKernelGGL(paged_join_kernel<T>, dim3(grid, cdiv(a.rows, JOIN_HEADS)), dim3(256), 0, stream, a);
     }

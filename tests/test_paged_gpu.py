@@ -260,6 +260,23 @@ def test_attention_of_large_batches_matches_the_oracle(dev, dtype, kvh, lens, pa
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("page", [8, 16])
+@pytest.mark.parametrize("heads", [(8, 8), (20, 1)])
+@pytest.mark.parametrize("longest, wide", [(120, 0), (120, 20000), (1700, 0), (1700, 20000), (6000, 0)])
+def test_attention_of_thousands_of_segments(dev, dtype, page, heads, longest, wide):
+    """More requests x key heads than run at once: short ones a wave each, long ones among them, in narrow tables and in tables far wider than any
+    length (other ways of dividing the work: the result is the same)."""
+    h, kvh = heads
+    R = 2063 // kvh if kvh > 1 else 1031
+    lens = [(i * 37) % 121 for i in range(R)]
+    lens[5], lens[R - 1], lens[R // 2] = longest, longest - 3, 0
+    kp, vp, table, lens = _cache(dev, lens, kvh, page, dtype, seed=page)
+    if wide:
+        table = torch.cat([table, torch.full((R, wide // page - table.shape[1]), -1, dtype=torch.int32)], 1)
+    _check(dev, torch.randn(R, h, 64, generator=torch.Generator().manual_seed(3)).to(dtype), kp, vp, table, lens, _slopes(h) / 8)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("scale", [0.0, 1e-30, -0.125, 1e-12, 3.0])
 def test_attention_with_any_scale(dev, dtype, scale):
     kp, vp, table, lens = _cache(dev, [300, 5, 0], 2, 8, dtype)
