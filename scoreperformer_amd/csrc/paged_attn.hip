@@ -50,7 +50,9 @@ struct PagedAttnArgs {
     int max_tiles;             // most tiles of a part
     int once;                  // whole segments: do not keep the rows in the caches (cut ones: decided on the device)
     int units;                 // room for this many parts
-    float* part; float* ml; int4* hdr;   // [units][rows][64], [units][rows][2], {parts of the batch}, [units] {request, key head and pass, parts (its first part only), 0}
+    float* part; float* ml;    // [units][rows][64], [units][rows][2]
+    int4* hdr;                 // {parts of the batch, most tiles of one, once, 0}, [units] {request, key head and pass, parts (its first part only), 0}
+    int* line;                 // batches of more than SEARCH requests: [R] parts of the requests before this one}
 };
 
 // reductions over the four lanes of a head (l, l ^ 16, l ^ 32, l ^ 48): the swapped halves of two copies, no LDS crossbar
@@ -429,18 +431,20 @@ __device__ __forceinline__ void do_part(const PagedAttnArgs& a, char (*smem)[2 *
 }
 
 // Four parts by four waves: a wave each where all are short, otherwise one after the other by all four.  A short part costs its latency, not its
-// bytes: 8000 segments of up to 100 rows 104 -> 55 us.
+// bytes: 8000 segments of up to 100 rows 112 -> 55 us.
 constexpr int SHORT = 24;   // tiles
 template <typename T, typename At, typename Done>
-__device__ __forceinline__ void do_four(const PagedAttnArgs& a, char (*smem)[2 * STAGE], int tid, int u, int all, bool once, const At& at, const Done& done) {
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int longest = 0;
-    for (int k = 0; k < 4 && u + k < all; ++k) { const Part p = at(u + k); longest = max(longest, p.t1 - p.t0); }
-    if (longest <= SHORT) {
+__device__ __forceinline__ void do_four(const PagedAttnArgs& a, char (*smem)[2 * STAGE], int* tiles, int tid, int u, int all, bool once, const At& at,
+                                        const Done& done) {
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), own = min(u + w, all - 1);
+    const Part mine = at(own);
+    if ((tid & 63) == 0) tiles[w] = mine.t1 - mine.t0;
+    __syncthreads();
+    const int longest = max(max(tiles[0], tiles[1]), max(tiles[2], tiles[3]));
+    if (__builtin_amdgcn_readfirstlane(longest) <= SHORT) {
         if (u + w < all) {
-            const Part p = at(u + w);
-            do_part<T, 1>(a, smem + w, tid & 63, p, once, p.parts > 1 ? u + w : -1);
-            if ((tid & 63) == 0) done(u + w, p);
+            do_part<T, 1>(a, smem + w, tid & 63, mine, once, mine.parts > 1 ? own : -1);
+            if ((tid & 63) == 0) done(own, mine);
         }
     } else {
         for (int k = 0; k < 4 && u + k < all; ++k) {
@@ -460,56 +464,109 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_whole_kernel(PagedAt
     do_part<T, WAVES>(a, smem, threadIdx.x, Part{r, n, (int)blockIdx.x - r * H, 0, tiles_in<T>(n), 0, 1}, a.once, -1);
 }
 
-// Segments cut into parts.  Every wave adds up the batch's tiles for itself (a lane: every 64th stretch of requests; no barrier, no LDS) and takes a
-// TARGET-th of them as the longest part; the parts of all segments stand in one line, of which workgroup g takes number g, g + G, ...  (four at a
-// time where there are enough of them).
+__device__ __forceinline__ int most_of(long total, int max_tiles) { return (int)min(max((long)MIN_TILES, (total + TARGET - 1) / TARGET), (long)max_tiles); }
+
+// Many requests: the line of parts by one workgroup in front, instead of by every wave (in wide tables, by every wave / in front: 16384 requests
+// of up to 100 rows 343 / 95 us, 4096 82 / 29, 500 15.0 / 11.5, 256 of up to 1000 19.1 / 20.8: hence SEARCH).
+constexpr int SEARCH = 256, LINE_T = 1024;
 template <typename T>
+__global__ __launch_bounds__(LINE_T) void paged_line_kernel(PagedAttnArgs a) {
+    __shared__ long s_sum[LINE_T / 64];
+    __shared__ int s_end[2][LINE_T / 64];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, H = a.kvh * a.passes;
+    long mine = 0;
+#pragma unroll 4
+    for (int r = tid; r < a.R; r += LINE_T) mine += tiles_in<T>(rows_at(a, r));
+#pragma unroll
+    for (int d = 32; d; d >>= 1) mine += __shfl_xor(mine, d, 64);
+    if (lane == 0) s_sum[w] = mine;
+    __syncthreads();
+    long total = 0;
+    for (int i = 0; i < LINE_T / 64; ++i) total += s_sum[i];
+    total *= H;
+    const int most = most_of(total, a.max_tiles);
+    int carry = 0;   // (the same in all threads)
+    for (int r0 = 0, k = 0; r0 < a.R; r0 += LINE_T, k ^= 1) {
+        const int r = r0 + tid, here = r < a.R ? H * parts_of(tiles_in<T>(rows_at(a, r)), most) : 0, to = wave_scan(here);
+        if (lane == 63) s_end[k][w] = to;
+        __syncthreads();   // (one a round: the other half of s_end is still being read)
+        int before = 0, round = 0;
+        for (int i = 0; i < LINE_T / 64; ++i) { const int e = s_end[k][i]; before += i < w ? e : 0; round += e; }
+        if (r < a.R) a.line[r] = carry + before + to - here;
+        carry += round;
+    }
+    if (tid == 0) a.hdr[0] = int4{min(carry, a.units), most, total * STAGE >= ONCE, total <= (long)carry * (SHORT / 2)};
+}
+
+// Segments cut into parts: a TARGET-th of the batch's tiles is the longest part, the parts of all segments stand in one line, of which workgroup g takes
+// number g, g + G, ...  (four at a time where there are enough of them, and short).  SEARCHED: the line was drawn by the kernel above; otherwise
+// every wave draws it for itself (a lane: every 64th stretch of requests; no barrier, no LDS, no launch).
+template <typename T, bool SEARCHED>
 __global__ __launch_bounds__(256, 2) void paged_attn_cut_kernel(PagedAttnArgs a) {
     __shared__ __attribute__((aligned(1024))) char smem[4][2 * STAGE];
+    __shared__ int s_tiles[4];
     const int tid = threadIdx.x, lane = tid & 63, H = a.kvh * a.passes;
-    const int per = (a.R + 63) / 64, q0 = min(a.R, lane * per), q1 = min(a.R, q0 + per);   // this lane's requests
-    const int first = q0 < q1 ? rows_at(a, q0) : 0;
-    long mine = tiles_in<T>(first);
-    for (int q = q0 + 1; q < q1; ++q) mine += tiles_in<T>(rows_at(a, q));
-    // in two halves of 32 bits: table capacities pass 2^32 tiles before memory does
-    const long total = H * (((long)__builtin_amdgcn_readlane(wave_scan((int)(mine >> 16)), 63) << 16) +
-                            (uint32_t)__builtin_amdgcn_readlane(wave_scan((int)(mine & 0xffff)), 63));
-    const int most = (int)min(max((long)MIN_TILES, (total + TARGET - 1) / TARGET), (long)a.max_tiles);
-    const bool once = total * STAGE >= ONCE;
-    int units = q0 < q1 ? H * parts_of(tiles_in<T>(first), most) : 0;
-    for (int q = q0 + 1; q < q1; ++q) units += H * parts_of(tiles_in<T>(rows_at(a, q)), most);
-    const int incl = wave_scan(units), all = min(__builtin_amdgcn_readlane(incl, 63), a.units);
-    if (blockIdx.x == 0 && tid == 0) a.hdr[0] = int4{all, 0, 0, 0};
+    const int per = (a.R + 63) / 64;
+    int all, most, first = 0, incl = 0, units = 0;
+    bool once, is_short;
+    if constexpr (SEARCHED) {
+        const int4 head = a.hdr[0];
+        all = __builtin_amdgcn_readfirstlane(head.x); most = __builtin_amdgcn_readfirstlane(head.y);
+        once = __builtin_amdgcn_readfirstlane(head.z); is_short = __builtin_amdgcn_readfirstlane(head.w);
+    } else {
+        const int q0 = min(a.R, lane * per), q1 = min(a.R, q0 + per);   // this lane's requests
+        first = q0 < q1 ? rows_at(a, q0) : 0;
+        long mine = tiles_in<T>(first);
+        for (int q = q0 + 1; q < q1; ++q) mine += tiles_in<T>(rows_at(a, q));
+        // in two halves of 32 bits: table capacities pass 2^32 tiles before memory does
+        const long total = H * (((long)__builtin_amdgcn_readlane(wave_scan((int)(mine >> 16)), 63) << 16) +
+                                (uint32_t)__builtin_amdgcn_readlane(wave_scan((int)(mine & 0xffff)), 63));
+        most = most_of(total, a.max_tiles);
+        once = total * STAGE >= ONCE;
+        units = q0 < q1 ? H * parts_of(tiles_in<T>(first), most) : 0;
+        for (int q = q0 + 1; q < q1; ++q) units += H * parts_of(tiles_in<T>(rows_at(a, q)), most);
+        incl = wave_scan(units);
+        all = min(__builtin_amdgcn_readlane(incl, 63), a.units);
+        is_short = total <= (long)all * (SHORT / 2);
+        if (blockIdx.x == 0 && tid == 0) a.hdr[0] = int4{all, 0, 0, 0};
+    }
     const auto at = [&](int u) {
         Part p;
-        const int from = __builtin_ctzll(__ballot(incl > u));
-        int off = u - __builtin_amdgcn_readlane(incl - units, from);
-        p.r = from * per; p.n = __builtin_amdgcn_readlane(first, from);
-        // more than 64 requests: those of the lane that was found, 64 at a time, a lane each
-        for (int base = p.r; per > 1; base += 64) {
-            const int q = base + lane, mine = q < min((from + 1) * per, a.R) ? rows_at(a, q) : 0;
-            const int here = q < min((from + 1) * per, a.R) ? H * parts_of(tiles_in<T>(mine), most) : 0, to = wave_scan(here);
-            const unsigned long long found = __ballot(to > off);
-            const bool last = base + 64 >= min((from + 1) * per, a.R);
-            if (found || last) {
-                const int k = found ? __builtin_ctzll(found) : 0;
-                p.r = base + k; p.n = __builtin_amdgcn_readlane(mine, k);
-                off -= __builtin_amdgcn_readlane(to - here, k);
-                break;
+        int off = u;
+        if constexpr (SEARCHED) {   // the last request that begins at or before u: 64 candidates at a time
+            int base = 0, span = a.R;
+            while (span > 1) {
+                const int step = (span + 63) >> 6;
+                const bool in = lane * step < span;
+                const int from = a.line[base + (in ? lane * step : 0)], k = 63 - __builtin_clzll(__ballot(in && from <= u) | 1);
+                base += k * step; span = min(step, span - k * step);
             }
-            off -= __builtin_amdgcn_readlane(to, 63);
+            p.r = base; p.n = __builtin_amdgcn_readfirstlane(rows_at(a, base)); off -= __builtin_amdgcn_readfirstlane(a.line[base]);
+        } else {
+            const int from = __builtin_ctzll(__ballot(incl > u));
+            off -= __builtin_amdgcn_readlane(incl - units, from);
+            p.r = from * per; p.n = __builtin_amdgcn_readlane(first, from);
+            // more than 64 requests: those of the lane that was found, a lane each (SEARCH / 64 at most)
+            if (per > 1) {
+                const int q = p.r + lane, rows = lane < per && q < a.R ? rows_at(a, q) : 0;
+                const int here = lane < per && q < a.R ? H * parts_of(tiles_in<T>(rows), most) : 0, to = wave_scan(here);
+                const unsigned long long found = __ballot(to > off);
+                const int k = found ? __builtin_ctzll(found) : 0;
+                p.r += k; p.n = __builtin_amdgcn_readlane(rows, k);
+                off -= __builtin_amdgcn_readlane(to - here, k);
+            }
         }
         p.parts = parts_of(tiles_in<T>(p.n), most);
         // (the bounds hold by themselves unless the lengths change while this runs; then the result is lost, but no access goes astray)
-        p.hp = min(off / p.parts, H - 1); p.part = min(off - p.hp * p.parts, p.parts - 1);
+        p.hp = max(0, min(off / p.parts, H - 1)); p.part = max(0, min(off - p.hp * p.parts, p.parts - 1));
         const int tiles = tiles_in<T>(p.n);
         p.t0 = (int)((long)tiles * p.part / p.parts); p.t1 = (int)((long)tiles * (p.part + 1) / p.parts);
         return p;
     };
     const auto done = [&](int u, const Part& p) { a.hdr[1 + u] = int4{p.r, p.hp, p.part == 0 && p.parts > 1 ? p.parts : 0, 0}; };
-    if (all >= 4 * RESIDENT && total <= (long)all * (SHORT / 2)) {
+    if (all >= 4 * RESIDENT && is_short) {
         for (int u = 4 * blockIdx.x; u < all; u += 4 * gridDim.x) {
-            do_four<T>(a, smem, tid, u, all, once, at, done);
+            do_four<T>(a, smem, s_tiles, tid, u, all, once, at, done);
             __syncthreads();   // the tiles of the next parts go where these results were
         }
     } else {
@@ -620,7 +677,10 @@ int page_shift(int page) {
     return -1;
 }
 
-size_t scratch_of(const Split& s) { return s.waves ? 0 : (size_t)s.units * ((size_t)s.rows * (HEAD + 2) * sizeof(float) + sizeof(int4)) + sizeof(int4); }
+size_t scratch_of(const Split& s, int R) {
+    if (s.waves) return 0;
+    return (size_t)s.units * ((size_t)s.rows * (HEAD + 2) * sizeof(float) + sizeof(int4)) + sizeof(int4) + (R > SEARCH ? R * sizeof(int) : 0);
+}
 
 template <typename T, int WAVES>
 void launch_whole(const PagedAttnArgs& a, long segments, hipStream_t stream) {
@@ -633,7 +693,11 @@ int launch(const PagedAttnArgs& a, const Split& s, hipStream_t stream) {
     else if (s.waves == 2) launch_whole<T, 2>(a, s.units, stream);
     else {
         const unsigned grid = s.units < GRID ? (unsigned)s.units : GRID;
-        hipLaunchKernelGGL(paged_attn_cut_kernel<T>, dim3(grid), dim3(256), 0, stream, a);
+        if (a.R > SEARCH) {
+            hipLaunchKernelGGL(paged_line_kernel<T>, dim3(1), dim3(LINE_T), 0, stream, a);
+            SPN_LAUNCH_CHECK();
+            hipLaunchKernelGGL((paged_attn_cut_kernel<T, true>), dim3(grid), dim3(256), 0, stream, a);
+        } else hipLaunchKernelGGL((paged_attn_cut_kernel<T, false>), dim3(grid), dim3(256), 0, stream, a);
         SPN_LAUNCH_CHECK();
         hipLaunchKernelGGL(paged_join_kernel<T>, dim3(grid, cdiv(a.rows, JOIN_HEADS)), dim3(256), 0, stream, a);
     }
@@ -646,7 +710,7 @@ int launch(const PagedAttnArgs& a, const Split& s, hipStream_t stream) {
 extern "C" size_t spn_paged_attn_workspace_bytes(int R, int h, int kvh, int W, int page, int dtype) {
     const int shift = page_shift(page);
     if (shift < 0 || R < 1 || h < 1 || kvh < 1 || h % kvh || W < 1) return 0;   // refused by the call itself
-    return scratch_of(split_of(R, h, kvh, W, shift, dtype == 1 ? 2 : 4));
+    return scratch_of(split_of(R, h, kvh, W, shift, dtype == 1 ? 2 : 4), R);
 }
 
 extern "C" int spn_paged_attn(const void* q, long q_rs, long q_hs, const void* k_pages, const void* v_pages, int dtype, const int* block_table, long bt_ld,
@@ -660,11 +724,11 @@ extern "C" int spn_paged_attn(const void* q, long q_rs, long q_hs, const void* k
                 (long)R * h < (1L << 21) && ((long)kvh * HEAD * 4 << shift) < (1L << 32), "spn_paged_attn: bad sizes");
     SPN_REQUIRE(((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) == 0, "spn_paged_attn: pages must be 16-byte aligned");
     const Split s = split_of(R, h, kvh, W, shift, dtype == 1 ? 2 : 4);
-    const size_t need = scratch_of(s);
+    const size_t need = scratch_of(s, R);
     SPN_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                 "spn_paged_attn: the workspace is too small or not 16-byte aligned (spn_paged_attn_workspace_bytes)");
     PagedAttnArgs a{q, q_rs, q_hs, k_pages, v_pages, block_table, bt_ld, lens, slopes, o, o_rs, o_hs, R, h, kvh, W, num_pages, shift, scale,
-                    h / kvh, s.passes, s.rows, s.max_tiles, s.once, (int)s.units, nullptr, nullptr, nullptr};
-    if (need) { a.hdr = (int4*)workspace; a.part = (float*)(a.hdr + 1 + s.units); a.ml = a.part + s.units * s.rows * HEAD; }
+                    h / kvh, s.passes, s.rows, s.max_tiles, s.once, (int)s.units, nullptr, nullptr, nullptr, nullptr};
+    if (need) { a.hdr = (int4*)workspace; a.part = (float*)(a.hdr + 1 + s.units); a.ml = a.part + s.units * s.rows * HEAD; a.line = (int*)(a.ml + s.units * s.rows * 2); }
     return dtype == 1 ? launch<bf16_t>(a, s, stream) : launch<float>(a, s, stream);
 }

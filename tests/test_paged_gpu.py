@@ -277,6 +277,18 @@ def test_attention_of_thousands_of_segments(dev, dtype, page, heads, longest, wi
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("R, h, kvh", [(256, 2, 1), (257, 2, 1), (512, 2, 1), (1025, 34, 2), (4097, 2, 2), (9000, 1, 1)])
+def test_attention_of_thousands_of_requests_in_wide_tables(dev, dtype, R, h, kvh):
+    """The line of parts over more requests than a wave, a workgroup, 64 x 64 searches hold; cut requests first, last and in between."""
+    lens = [(i * 29) % 41 for i in range(R)]
+    for i, n in ((0, 5000), (R - 1, 900), (R // 2, 2500), (63, 700), (64, 701)):
+        lens[i] = n
+    kp, vp, table, lens = _cache(dev, lens, kvh, 16, dtype, seed=R)
+    table = torch.cat([table, torch.full((R, 1300 - table.shape[1]), -1, dtype=torch.int32)], 1)
+    _check(dev, torch.randn(R, h, 64, generator=torch.Generator().manual_seed(4)).to(dtype), kp, vp, table, lens, _slopes(h) / 8)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("scale", [0.0, 1e-30, -0.125, 1e-12, 3.0])
 def test_attention_with_any_scale(dev, dtype, scale):
     kp, vp, table, lens = _cache(dev, [300, 5, 0], 2, 8, dtype)
