@@ -37,7 +37,7 @@ class PagedStep:
 
 class PagedKVCache:
     """`stack`: the decoder (`Transformer`, causal, self-attention only) whose layers it serves.  One pool of `num_pages` pages of `page_size` rows per
-    layer, the same page ids for all layers; `max_len`: rows a request can hold; bf16, like the operands of the attention kernels."""
+    layer, the same page ids for all layers; `max_len`: rows a request can hold, rounded up to whole pages; bf16, like the operands of the attention kernels."""
 
     def __init__(self, stack, num_pages: int, max_requests: int, max_len: int, page_size: int = 16, device=None):
         blocks = [layer[1] for kind, layer in zip(stack.layer_types, stack.layers) if kind == "a"]
@@ -65,6 +65,8 @@ class PagedKVCache:
         """Room for new [R] (int32, on the device) more rows per request, at most `width` each.  width > 1 is the prompt form: its rows attend to each
         other only, so a request that already holds rows takes none (its count is refused).  A request that cannot be served whole -- no pages left,
         more than `max_len` rows -- takes none either: its slots are -1, its length stays, and the attention adds nothing to its rows (step.mask tells)."""
+        if new.shape != self.lens.shape:
+            raise ValueError(f"new rows of {list(new.shape)} for {self.max_requests} requests")
         if width > 1:
             new = torch.where((self.lens == 0) | (new == 0), new, -1)
         slots, _, _ = ops.paged_plan(self.lens, new, self.block_table, self.free_pages, self.num_free, self.page_size, width, lens_out=self.lens,

@@ -194,6 +194,9 @@ def test_paged_cache_refuses_what_it_does_not_serve():
         PagedKVCache(_stack(cross_attend=True), **ok)
     with pytest.raises(NotImplementedError, match="memory"):
         PagedKVCache(_stack(attention=AttentionConfig(num_mem_kv=2)), **ok)
+    for new in (torch.ones(1, dtype=torch.int32), torch.ones(2, 1, dtype=torch.int32)):     # (would broadcast)
+        with pytest.raises(ValueError, match="new rows"):
+            c.plan(new, width=4)
     for bad in (dict(num_pages=0), dict(max_requests=0), dict(max_len=0), dict(page_size=12), dict(page_size=4)):
         with pytest.raises(ValueError):
             PagedKVCache(_stack(), **{**ok, **bad})
