@@ -490,3 +490,36 @@ def test_a_decode_step_captured_and_replayed(dev):
                     sc = torch.einsum("jhd,hd->hj", kv[:, 0], row[r, :h * 64].double().view(h, 64)) / 8 + _slopes(h).double()[:, None] * torch.arange(1 - n, 1).double()
                     want[r] = torch.einsum("hj,jhd->hd", torch.softmax(sc, 1), kv[:, 1])
             assert float((c.out.cpu().double() - want).abs().max()) <= 2.0 ** -8 * 5, it       # |o| <= max |v| < 5: one rounding of the output
+
+
+@pytest.mark.parametrize("R", [3, 300])
+def test_graphs_of_cut_batches_replayed_at_once(dev, R):
+    """Captured calls in tables far wider than the lengths (cut segments, the line drawn by every wave / in front): each replay divides the lengths that
+    are there then, and two graphs in flight on two streams have scratch of their own."""
+    ops, rng = _ops(), np.random.default_rng(R)
+    calls = []
+    for seed in (1, 2):
+        kp, vp, table, lens = _cache(dev, [2100] * 3 + [40] * (R - 3), 2, 16, BF16, seed=seed)
+        table = torch.cat([table, torch.full((R, 1500), -1, dtype=torch.int32)], 1)
+        d = [x.to(dev) for x in (torch.randn(R, 8, 64).to(BF16), kp, vp, table, lens)]
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            ops.paged_attn(*d)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.paged_attn(*d)
+        calls.append((s, g, d, out))
+    for it in range(8):
+        for _, _, d, _ in calls:
+            n = rng.integers(0, 41, R)
+            n[:3] = rng.integers(0, 2101, 3)
+            d[4].copy_(torch.from_numpy(n).int())
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for s, g, _, _ in calls:
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for _, _, d, out in calls:
+            assert torch.equal(out, ops.paged_attn(*d)), it
