@@ -85,17 +85,17 @@ __device__ __forceinline__ void dma(uint32_t lds, const uint32_t* off, const cha
         else asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off[0]), "s"(base) : "memory");
     } else if constexpr (N == 2) {
         if constexpr (NT)
-            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %3 nt\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024 nt"
+            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %3 nt\n\tglobal_load_lds_dwordx4 %2, %3 offset:0x400 nt"
                          :: "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
-        else asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" :: "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
+        else asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:0x400" :: "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
     } else {
         static_assert(N == 4, "pieces of one base");
         if constexpr (NT)
-            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %5 nt\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024 nt\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048 nt\n\t"
-                         "global_load_lds_dwordx4 %4, %5 offset:3072 nt" :: "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory");
+            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %5 nt\n\tglobal_load_lds_dwordx4 %2, %5 offset:0x400 nt\n\tglobal_load_lds_dwordx4 %3, %5 offset:0x800 nt\n\t"
+                         "global_load_lds_dwordx4 %4, %5 offset:0xc00 nt" :: "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory");
         else
-            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024\n\tglobal_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-                         "global_load_lds_dwordx4 %4, %5 offset:3072" :: "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory");
+            asm volatile(SPN_LEAD "global_load_lds_dwordx4 %1, %5\n\tglobal_load_lds_dwordx4 %2, %5 offset:0x400\n\tglobal_load_lds_dwordx4 %3, %5 offset:0x800\n\t"
+                         "global_load_lds_dwordx4 %4, %5 offset:0xc00" :: "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory");
     }
 #undef SPN_LEAD
 }
