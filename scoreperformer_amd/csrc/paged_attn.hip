@@ -23,24 +23,19 @@
 // 57 us = 4.7 TB/s; 64 multi-query, 0 .. 2048 (17 MB): 10.4 us; one of 4096 rows (1 MB): 8.3 us in two launches, one of 256: 4.2 us in one.
 #include "common.h"
 #include "paged_index.h"
+#include "paged_split.h"
 
 using namespace spn_paged;
 
 namespace {
 
-constexpr int HEADS = 16;           // query heads of a segment
-constexpr int STAGE = 8192;         // bytes of a tile: 4 KiB of keys, 4 KiB of values
 constexpr int LDO = 68;             // LDS row of a head's o: 64 + 4, so that 16 heads do not meet in one bank
 constexpr float LOG2E_F = 1.4426950408889634f;
 constexpr float RISE = 8.f;         // log2: probabilities up to 2^8 of the reference are carried as they are
-constexpr int MIN_TILES = 4;        // least tiles of a part (a tile per wave; 2: the same, 8: 1 x 4096 rows 8.9 -> 8.2 us the other way)
-constexpr int TARGET = 512;         // parts the batch is cut into, beside one per segment (1024: the same within 2 %)
-constexpr int MAX_TILES = 64;       // most tiles of a part where the batch is larger (32: 256 x 4096 rows 182 -> 196 us, 128: 186)
-constexpr int RESIDENT = 512;       // workgroups of 4 waves that run at once: two on a compute unit, by their LDS
-constexpr unsigned GRID = 2 * RESIDENT;   // workgroups of a cut batch
-constexpr int MAX_PARTS = 128;      // parts of a segment (one of 131072 rows, 256: 18.9 us, 128: 17.2, 64: 20.8 when a tile cost a tenth more)
 
 template <typename T> constexpr int TILE = 64 / (int)sizeof(T);    // rows of a tile: 32 (bf16), 16 (fp32)
+
+static_assert(sizeof(int4) == HDR, "header of a part");
 
 struct PagedAttnArgs {
     const void* q; long q_rs, q_hs; const void* kp; const void* vp; const int* table; long ld; const int* lens; const float* slopes;
@@ -382,12 +377,6 @@ __device__ __forceinline__ int wave_scan(int v) {
 template <typename T> __device__ __forceinline__ int tiles_in(int rows) { return (rows + TILE<T> - 1) / TILE<T>; }
 __device__ __forceinline__ int rows_at(const PagedAttnArgs& a, int r) { return rows_of(a.lens[r], a.W, a.shift); }
 
-// parts of a segment of `tiles` tiles, none above `most` tiles unless there would be more than MAX_PARTS
-__device__ __forceinline__ int parts_of(int tiles, int most) { return max(1, min(MAX_PARTS, (int)(((uint32_t)tiles + (uint32_t)most - 1u) / (uint32_t)most))); }
-
-constexpr long ONCE = 64L << 20;   // bytes of rows from which they are not kept in the caches (Infinity Cache: 256 MiB; a step walks every layer's cache
-                                   // before it is back at this one).  1.07 GB: 195 -> 177 us; 17 MB, three pools in turn: 11.4 -> 13.3 us, hence the bound
-
 // tiles [t0, t1) of segment hp (key head and 16-head pass) of request r, which holds n rows; parts: into how many the segment is cut
 struct Part { int r, n, hp, t0, t1, part, parts; };
 
@@ -464,11 +453,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attn_whole_kernel(PagedAt
     do_part<T, WAVES>(a, smem, threadIdx.x, Part{r, n, (int)blockIdx.x - r * H, 0, tiles_in<T>(n), 0, 1}, a.once, -1);
 }
 
-__device__ __forceinline__ int most_of(long total, int max_tiles) { return (int)min(max((long)MIN_TILES, (total + TARGET - 1) / TARGET), (long)max_tiles); }
-
 // Many requests: the line of parts by one workgroup in front, instead of by every wave (in wide tables, by every wave / in front: 16384 requests
 // of up to 100 rows 343 / 95 us, 4096 82 / 29, 500 15.0 / 11.5, 256 of up to 1000 19.1 / 20.8: hence SEARCH).
-constexpr int SEARCH = 256, LINE_T = 1024;
+constexpr int LINE_T = 1024;
 template <typename T>
 __global__ __launch_bounds__(LINE_T) void paged_line_kernel(PagedAttnArgs a) {
     __shared__ long s_sum[LINE_T / 64];
@@ -642,44 +629,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     }
 }
 
-struct Split { long units; int waves; int passes, rows, max_tiles, once; };   // waves: of a workgroup that takes a whole segment; 0: cut
-Split split_of(int R, int h, int kvh, int W, int shift, int esize) {
-    Split s;
-    const int group = h / kvh;
-    s.passes = (group + HEADS - 1) / HEADS; s.rows = group < HEADS ? group : HEADS;
-    const long segments = (long)R * kvh * s.passes, cap = (long)W << shift, bytes = cap * HEAD * 2 * esize, tiles = (bytes + STAGE - 1) / STAGE;
-    // Whole segments, one launch instead of two: a lone workgroup of 8 waves reads 105 GB/s (fp32, bound by its matrix instructions: 56), the machine
-    // about 5 TB/s, the second launch costs some 6 us of device and host time, so with tables filled by half
-    //   bytes / rate  <=  segments * bytes / 2 / 5 TB/s + 6 us,
-    // and never where one full table among short ones would take long by itself (1 MiB: 10 us for 4096 rows of a bf16 key head, 19 for 2048 of fp32).
-    // Measured, whole / cut: 64 x 2048 rows 10.3 / 13.5 us, 1 x 4096 13.6 / 8.2, 16 x 512 5.1 / 8.2, 39 segments of 1001 fp32 rows 14.5 / 10.7,
-    // 2048 segments of up to 4096 rows 176 / 184.
-    const long rate = esize == 2 ? 105 : 56;   // bytes per ns
-    const bool whole = bytes <= (1L << 20) && bytes * (10000 - rate * segments) <= 6000 * rate * 10000;
-    // waves: 8 where the segments do not fill the machine.  Where they do, their lengths decide, which the host does not know: 8 waves serve long rows
-    // best (2048 segments of up to 4096 rows, 2 / 4 / 8 waves: 193, 180, 176 us), 2 waves short ones (8000 of up to 100: 30, 50, 89; 2048 of up to
-    // 500: 26, 28, 38; of up to 1000: 45, 43, 51), so the width of the tables is the hint and 8 is left out
-    s.waves = !whole ? 0 : segments >= 4 * RESIDENT ? (tiles > 64 ? 4 : 2) : segments > 256 ? 4 : tiles > 8 ? 8 : 4;
-    s.once = segments * bytes >= 2 * ONCE;   // tables filled by half
-    // the longest part: MAX_TILES, or what keeps the workspace -- all tables full -- to 8192 parts
-    const long full = segments * tiles, most = (full + 8191) / 8192;
-    s.max_tiles = (int)(most < MAX_TILES ? MAX_TILES : most);
-    // parts on the device: at most tiles / most + 1 for each segment, with most >= MIN_TILES and most >= min(max_tiles, all tiles / TARGET)
-    long units = full / s.max_tiles;
-    units = (units < TARGET ? TARGET : units) + segments;
-    const long finest = segments * ((tiles + MIN_TILES - 1) / MIN_TILES);
-    s.units = whole ? segments : units < finest ? units : finest;
-    return s;
-}
-
 int page_shift(int page) {
     for (int s = 3; s <= 12; ++s) if (page == 1 << s) return s;
     return -1;
-}
-
-size_t scratch_of(const Split& s, int R) {
-    if (s.waves) return 0;
-    return (size_t)s.units * ((size_t)s.rows * (HEAD + 2) * sizeof(float) + sizeof(int4)) + sizeof(int4) + (R > SEARCH ? R * sizeof(int) : 0);
 }
 
 template <typename T, int WAVES>
@@ -709,7 +661,7 @@ int launch(const PagedAttnArgs& a, const Split& s, hipStream_t stream) {
 
 extern "C" size_t spn_paged_attn_workspace_bytes(int R, int h, int kvh, int W, int page, int dtype) {
     const int shift = page_shift(page);
-    if (shift < 0 || R < 1 || h < 1 || kvh < 1 || h % kvh || W < 1) return 0;   // refused by the call itself
+    if (shift < 0 || !sizes_ok(R, h, kvh, W, shift)) return 0;   // refused by the call itself
     return scratch_of(split_of(R, h, kvh, W, shift, dtype == 1 ? 2 : 4), R);
 }
 
@@ -720,8 +672,7 @@ extern "C" int spn_paged_attn(const void* q, long q_rs, long q_hs, const void* k
     SPN_REQUIRE(q && k_pages && v_pages && block_table && lens && o, "spn_paged_attn: null buffer");
     SPN_REQUIRE(dtype == 0 || dtype == 1, "spn_paged_attn: dtype codes are 0 (fp32) and 1 (bf16)");
     SPN_REQUIRE(shift >= 0, "spn_paged_attn: the page size must be a power of two in [8, 4096]");
-    SPN_REQUIRE(R > 0 && h > 0 && kvh > 0 && h % kvh == 0 && W > 0 && num_pages > 0 && bt_ld >= W && ((long)W << shift) < (1L << 31) && (long)R * W < (1L << 31) &&
-                (long)R * h < (1L << 21) && ((long)kvh * HEAD * 4 << shift) < (1L << 32), "spn_paged_attn: bad sizes");
+    SPN_REQUIRE(num_pages > 0 && bt_ld >= W && sizes_ok(R, h, kvh, W, shift), "spn_paged_attn: bad sizes");
     SPN_REQUIRE(((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15) == 0, "spn_paged_attn: pages must be 16-byte aligned");
     const Split s = split_of(R, h, kvh, W, shift, dtype == 1 ? 2 : 4);
     const size_t need = scratch_of(s, R);
