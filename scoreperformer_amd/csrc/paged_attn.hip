@@ -280,7 +280,7 @@ struct Walk {
         float p[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) p[e] = __builtin_fmaf(c1, s[e >> 2][e & 3], base);
-        if (t * TILE<T> + TILE<T> > n || pg.bad) {   // rows behind the length or on no page: no weight, and no bit of theirs in the product
+        if (part_filled(t, TILE<T>, n) || pg.bad) {   // rows behind the length or on no page: no weight, and no bit of theirs in the product
             const bool ok = !(pg.bad >> (g * E / UNIT) & 1);
 #pragma unroll
             for (int e = 0; e < E; ++e) p[e] = ok && row0 + e < n ? p[e] : -__builtin_inff();
@@ -374,7 +374,7 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
 
-template <typename T> __device__ __forceinline__ int tiles_in(int rows) { return (rows + TILE<T> - 1) / TILE<T>; }
+template <typename T> __device__ __forceinline__ int tiles_in(int rows) { return tiles_of(rows, TILE<T>); }
 __device__ __forceinline__ int rows_at(const PagedAttnArgs& a, int r) { return rows_of(a.lens[r], a.W, a.shift); }
 
 // tiles [t0, t1) of segment hp (key head and 16-head pass) of request r, which holds n rows; parts: into how many the segment is cut

@@ -20,6 +20,10 @@ constexpr size_t HDR = 16;          // bytes of a part's header
 constexpr long ONCE = 64L << 20;   // bytes of rows from which they are not kept in the caches (Infinity Cache: 256 MiB; a step walks every layer's cache
                                    // before it is back at this one).  1.07 GB: 195 -> 177 us; 17 MB, three pools in turn: 11.4 -> 13.3 us, hence the bound
 
+// tiles of `tile` rows that 0 .. 2^31 - 1 rows take, and whether tile t of them is not filled to its end: no sum passes the type
+SPN_HD int tiles_of(int rows, int tile) { return (int)(((uint32_t)rows + (uint32_t)tile - 1u) / (uint32_t)tile); }
+SPN_HD bool part_filled(int t, int tile, int rows) { return rows - t * tile < tile; }
+
 // parts of a segment of `tiles` tiles, none above `most` tiles unless there would be more than MAX_PARTS
 SPN_HD int parts_of(int tiles, int most) {
     const int parts = (int)(((uint32_t)tiles + (uint32_t)most - 1u) / (uint32_t)most);

@@ -73,6 +73,30 @@ def test_the_division_of_any_accepted_batch_fits_its_workspace(tmp_path):
     _host_check(tmp_path, SPLIT)
 
 
+TILES = HEAD + r"""
+int main() {
+    const int R = 1, h = 1, kvh = 1, shift = 3, W = 1, esize = 2;
+    for (int tile = 16; tile <= 32; tile *= 2)
+        for (int it = 0; it < 1000000; ++it) {
+            const int rows = it < 5000 ? it : it < 10000 ? INT_MAX - (it - 5000) : lg(2147483647.0);
+            const int n = tiles_of(rows, tile);
+            NEED(n >= 0 && (long)n * tile >= rows && (long)(n - 1) * tile < rows);
+            for (int t = n - 1; t >= 0 && t >= n - 3; --t) {                                // the kernel asks for tiles that hold a row
+                NEED(part_filled(t, tile, rows) == ((long)t * tile + tile > rows));
+                NEED((long)t * tile + tile - 1 <= INT_MAX);                                 // every row number of the tile is an int
+            }
+        }
+    std::puts("ok");
+    return 0;
+}
+"""
+
+
+def test_tiles_of_any_length(tmp_path):
+    """Lengths up to 2^31 - 1: as many tiles as hold the rows, and the last one known as such."""
+    _host_check(tmp_path, TILES)
+
+
 QUERY = """
 import ctypes, sys
 lib = ctypes.CDLL(sys.argv[1])
