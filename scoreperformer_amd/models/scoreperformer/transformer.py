@@ -101,19 +101,33 @@ class TupleTransformer(nn.Module, Constructor):
             assert self.token_emb.continuous, "TupleTokenRegressionHead depends on `continuous` token embeddings."
             self.regression_head = TupleTokenRegressionHead.init(config=regression_head, dim=dim)
 
+    def _check_paged_rows(self, step, x, x_extra, context, style):
+        """Everything per note holds the step's rows: a longer tensor would silently give every step the first notes of the sequence."""
+        extra = [x_extra] if isinstance(x_extra, Tensor) else list(x_extra or ())
+        given = [("x", x)] + [("x_extra", t) for t in extra if hasattr(self.token_emb, "multiseq_mode")]
+        if self.context_emb_mode == EmbeddingModes.CONCAT:
+            given.append(("context", context))
+        if style is not None and (self.style_emb_mode == EmbeddingModes.CONCAT or style.shape[1] != 1):
+            given.append(("style_embeddings", style))
+        for name, t in given:
+            if t is not None and t.shape[:2] != step.slots.shape:
+                raise ValueError(f"{name} {list(t.shape)} does not hold the rows of the paged step {list(step.slots.shape)}")
+
     @no_autocast
     def forward(self, x: Tensor, mask: Optional[Tensor] = None, x_extra=None, style_embeddings: Optional[Tensor] = None,
                 context: Optional[Tensor] = None, context_mask: Optional[Tensor] = None,
                 caches: Optional[TupleTransformerCaches] = None, logits_keys: Optional[List] = None,
                 return_embeddings: bool = False, return_attn: bool = False, return_caches: bool = False,
                 labels: Optional[Tensor] = None, want_argmax: bool = False, label_counts=None, paged=None, **kwargs):
-        """`paged`: a step of a PagedKVCache made for `self.transformer`; x [R, width, dims] are the new notes of every request, context / style
-        embeddings theirs alone.  The caches of the reference's protocol (`caches`, `return_caches`) do not go with it."""
+        """`paged`: a step of a PagedKVCache made for `self.transformer`; x [R, width, dims] are the new notes of every request, x_extra, context and
+        style embeddings theirs alone (not those of the whole sequence; an adaptive style may be one row per request).  The caches of the
+        reference's protocol (`caches`, `return_caches`) do not go with it."""
         if paged is not None:
             if caches is not None or return_caches or mask is not None:
                 raise ValueError("a paged step brings its own mask and cache")
             if self.pos_emb is not None:
                 raise NotImplementedError("paged steps with absolute position embeddings: the notes' positions are on the device")
+            self._check_paged_rows(paged, x, x_extra, context, style_embeddings)
         token_emb_cache = caches.token_emb if caches is not None else None
         if hasattr(self.token_emb, "multiseq_mode") and x_extra is not None:
             x_extra = [x_extra] if isinstance(x_extra, Tensor) else x_extra
