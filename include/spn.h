@@ -173,6 +173,12 @@ int spn_embed_fwd(int nkeys, const float* const* tables, const int* V, const int
 int spn_embed_bwd(int nkeys, const float* const* tables, float* const* dtables, const int* V, const int* E, const long* tokens,
                   long tok_bs, long tok_ts, int t_len, const void* dy, long lddy, const float* gamma, const float* mean,
                   const float* rstd, float* dgamma, float* dbeta, float* ws, int T, int padding_idx, spn_stream_t stream);
+/* spn_embed_bwd with dgamma / dbeta summed in a fixed order (spn_embed_bwd: by atomics; ws there: 2 T floats): the same bits every time.
+ * ws: ws_floats >= spn_embed_bwd_det_workspace_floats(T, sum of E) (it depends on the tuning knob embed_stats_blocks). */
+int spn_embed_bwd_det(int nkeys, const float* const* tables, float* const* dtables, const int* V, const int* E, const long* tokens,
+                      long tok_bs, long tok_ts, int t_len, const void* dy, long lddy, const float* gamma, const float* mean,
+                      const float* rstd, float* dgamma, float* dbeta, float* ws, long ws_floats, int T, int padding_idx, spn_stream_t stream);
+long spn_embed_bwd_det_workspace_floats(int T, int D);
 
 /* ---- losses (models/scoreperformer/wrappers.py:49-59 CE; mmd_transformer.py:325-368 segments, 505-534 MMD) */
 int spn_ce_fwd(const void* logits, int dtype, long ld, const long* labels, long lab_bs, long lab_ts, int t_len,

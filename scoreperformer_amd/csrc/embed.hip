@@ -273,14 +273,15 @@ __global__ __launch_bounds__(256) void embed_fwd_wide_kernel(GatherDesc d, const
     }
 }
 
-// backward pass 1: per-row LN-backward sums s1 = mean(g), s2 = mean(g*xhat) with g = dy*gamma, and dgamma/dbeta.
+// backward pass 1: per-row LN-backward sums s1 = mean(g), s2 = mean(g*xhat) with g = dy*gamma, and dgamma/dbeta: the block's column sums into
+// part [blocks][dgamma | dbeta] (added up by embed_bwd_colsum_kernel), or, where part is null, by atomics.
 template <int NV>
 __global__ __launch_bounds__(256) void embed_bwd_stats_kernel(GatherDesc d, const long* __restrict__ tokens, long tok_bs, long tok_ts, int t_len,
                                                               const bf16_t* __restrict__ dy, long lddy, const float* __restrict__ gamma,
                                                               const float* __restrict__ mean, const float* __restrict__ rstd,
                                                               float* __restrict__ s1o, float* __restrict__ s2o,
-                                                              float* __restrict__ dgamma, float* __restrict__ dbeta, int T,
-                                                              int rows_per_block) {
+                                                              float* __restrict__ dgamma, float* __restrict__ dbeta, float* __restrict__ part,
+                                                              int T, int rows_per_block) {
     __shared__ float red[4][64 * NV * 4 + 4];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     f32x4 pg[NV], pb[NV];
@@ -357,9 +358,34 @@ __global__ __launch_bounds__(256) void embed_bwd_stats_kernel(GatherDesc d, cons
 #pragma unroll
             for (int e = 0; e < 4; ++e) red[w][(lane + 64 * i) * 4 + e] = pass == 0 ? pg[i][e] : pb[i][e];
         __syncthreads();
-        for (int col = threadIdx.x; col < d.D; col += 256)
-            atomicAdd((pass == 0 ? dgamma : dbeta) + col, red[0][col] + red[1][col] + red[2][col] + red[3][col]);
+        for (int col = threadIdx.x; col < d.D; col += 256) {
+            const float sum = red[0][col] + red[1][col] + red[2][col] + red[3][col];
+            if (part) part[((long)blockIdx.x * 2 + pass) * d.D + col] = sum;
+            else atomicAdd((pass == 0 ? dgamma : dbeta) + col, sum);
+        }
         __syncthreads();
+    }
+}
+
+// The blocks' column sums added up, for every column in the same order: an element of dgamma whose terms cancel is otherwise noise of 1 % of itself
+// from run to run.  32 columns a workgroup, 32 threads a column, one add into the gradient.  Whole backward at 12 keys x 128, by atomics / in
+// order: 132 notes 19.0 / 21.0 us (a launch more), 4097 78.2 / 67.8, 131072 391 / 381 (2048 adds a column were the longer way).
+__global__ __launch_bounds__(1024) void embed_bwd_colsum_kernel(const float* __restrict__ part, int blocks, int D, float* __restrict__ dgamma,
+                                                                float* __restrict__ dbeta) {
+    __shared__ float red[32][33];
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
+    float sum = 0.f;
+    if (col < 2 * D) {
+#pragma unroll 8
+        for (int b = g; b < blocks; b += 32) sum += part[(long)b * 2 * D + col];
+    }
+    red[g][c] = sum;
+    __syncthreads();
+    if (g == 0 && col < 2 * D) {
+        sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) sum += red[k][c];
+        atomicAdd(col < D ? dgamma + col : dbeta + (col - D), sum);
     }
 }
 
@@ -682,10 +708,16 @@ extern "C" int spn_embed_fwd(int nkeys, const float* const* tables, const int* V
     return SPN_OK;
 }
 
-// dtables (fp32 [V,E] per key) and dgamma/dbeta are ACCUMULATED.  ws: 2*T floats of workspace.
-extern "C" int spn_embed_bwd(int nkeys, const float* const* tables, float* const* dtables, const int* V, const int* E,
-                             const long* tokens, long tok_bs, long tok_ts, int t_len, const void* dy, long lddy, const float* gamma, const float* mean,
-                             const float* rstd, float* dgamma, float* dbeta, float* ws, int T, int padding_idx, hipStream_t stream) {
+// rows of a block of the statistics pass
+static int stats_rows(int T) {
+    const int blocks = spn_tune_i(SPN_TUNE_EMBED_STATS_BLOCKS) > 0 ? spn_tune_i(SPN_TUNE_EMBED_STATS_BLOCKS) : 2048;   // tuning aid (2048: -5 % over 1024; 256 or 16384: slower)
+    return (cdiv(T, blocks) + 3) / 4 * 4;
+}
+
+// ws: s1, s2 [T] and, with `ordered`, the blocks' column sums behind them
+static int embed_bwd(int nkeys, const float* const* tables, float* const* dtables, const int* V, const int* E, const long* tokens, long tok_bs,
+                     long tok_ts, int t_len, const void* dy, long lddy, const float* gamma, const float* mean, const float* rstd, float* dgamma,
+                     float* dbeta, float* ws, bool ordered, int T, int padding_idx, hipStream_t stream) {
     SPN_REQUIRE(nkeys > 0 && nkeys <= MAXK && tokens && dy && dtables && T > 0, "spn_embed_bwd: bad arguments");
     GatherDesc d;
     const int D = fill_gather(d, nkeys, tables, dtables, V, E);
@@ -694,15 +726,17 @@ extern "C" int spn_embed_bwd(int nkeys, const float* const* tables, float* const
     if (gamma) {
         SPN_REQUIRE(mean && rstd && dgamma && dbeta && ws, "spn_embed_bwd: LayerNorm buffers required with gamma");
         const int nv = round_nv((D + 255) / 256);
-        const int stats_blocks = spn_tune_i(SPN_TUNE_EMBED_STATS_BLOCKS) > 0 ? spn_tune_i(SPN_TUNE_EMBED_STATS_BLOCKS) : 2048;   // tuning aid (2048: -5 % over 1024; 256 or 16384: slower)
-        int rpb = cdiv(T, stats_blocks); rpb = ((rpb + 3) / 4) * 4;
-        // a few short sequences: one block, so that dgamma / dbeta take ONE atomic add per column and do not depend on the order of blocks
-        // (an element whose terms cancel is otherwise noise of 1 % of itself from run to run; at these sizes the pass is launch-bound)
-        if (T <= 128) rpb = 128;
+        const int rpb = stats_rows(T);
         dim3 grid(cdiv(T, rpb));
-#define CASE(NV_) case NV_: hipLaunchKernelGGL((embed_bwd_stats_kernel<NV_>), grid, dim3(256), 0, stream, d, tokens, tok_bs, tok_ts, t_len, (const bf16_t*)dy, lddy, gamma, mean, rstd, s1, s2, dgamma, dbeta, T, rpb); break;
+        float* part = ordered && grid.x > 1 ? ws + 2L * T : nullptr;   // (one block: one add per column)
+#define CASE(NV_) case NV_: hipLaunchKernelGGL((embed_bwd_stats_kernel<NV_>), grid, dim3(256), 0, stream, d, tokens, tok_bs, tok_ts, t_len, (const bf16_t*)dy, lddy, gamma, mean, rstd, s1, s2, dgamma, dbeta, part, T, rpb); break;
         switch (nv) { CASE(1) CASE(2) CASE(4) CASE(6) CASE(8) default: return SPN_ERR_ARG; }
 #undef CASE
+        if (part) {
+            SPN_LAUNCH_CHECK();
+            hipLaunchKernelGGL(embed_bwd_colsum_kernel, dim3(cdiv(2 * D, 32)), dim3(1024), 0, stream, part, (int)grid.x, D, dgamma, dbeta);
+            SPN_LAUNCH_CHECK();
+        }
     }
     bool mfma_ok = lddy % 8 == 0 && (((uintptr_t)dy) & 15) == 0;
     for (int i = 0; i < nkeys; ++i) mfma_ok = mfma_ok && E[i] == 128 && V[i] <= 512;
@@ -736,4 +770,29 @@ extern "C" int spn_embed_bwd(int nkeys, const float* const* tables, float* const
                             (const bf16_t*)dy, lddy, gamma, mean, rstd, s1, s2, T, rpb, padding_idx);
     SPN_LAUNCH_CHECK();
     return SPN_OK;
+}
+
+// dtables (fp32 [V,E] per key) and dgamma/dbeta are ACCUMULATED.  ws: 2*T floats of workspace.
+extern "C" int spn_embed_bwd(int nkeys, const float* const* tables, float* const* dtables, const int* V, const int* E,
+                             const long* tokens, long tok_bs, long tok_ts, int t_len, const void* dy, long lddy, const float* gamma, const float* mean,
+                             const float* rstd, float* dgamma, float* dbeta, float* ws, int T, int padding_idx, hipStream_t stream) {
+    return embed_bwd(nkeys, tables, dtables, V, E, tokens, tok_bs, tok_ts, t_len, dy, lddy, gamma, mean, rstd, dgamma, dbeta, ws, false, T, padding_idx, stream);
+}
+
+extern "C" long spn_embed_bwd_det_workspace_floats(int T, int D) {
+    if (T < 1 || D < 1) return 0;
+    const int blocks = cdiv(T, stats_rows(T));
+    return 2L * T + (blocks > 1 ? 2L * blocks * D : 0);
+}
+
+// The same with dgamma / dbeta summed in a fixed order.  ws: ws_floats >= spn_embed_bwd_det_workspace_floats(T, sum E).
+extern "C" int spn_embed_bwd_det(int nkeys, const float* const* tables, float* const* dtables, const int* V, const int* E,
+                                 const long* tokens, long tok_bs, long tok_ts, int t_len, const void* dy, long lddy, const float* gamma, const float* mean,
+                                 const float* rstd, float* dgamma, float* dbeta, float* ws, long ws_floats, int T, int padding_idx, hipStream_t stream) {
+    SPN_REQUIRE(nkeys > 0 && nkeys <= MAXK && E && T > 0, "spn_embed_bwd_det: bad arguments");
+    long D = 0;
+    for (int i = 0; i < nkeys; ++i) D += E[i];
+    SPN_REQUIRE(!gamma || (D > 0 && D <= 2048 && ws && ws_floats >= spn_embed_bwd_det_workspace_floats(T, (int)D)),
+                "spn_embed_bwd_det: the workspace is too small (spn_embed_bwd_det_workspace_floats)");
+    return embed_bwd(nkeys, tables, dtables, V, E, tokens, tok_bs, tok_ts, t_len, dy, lddy, gamma, mean, rstd, dgamma, dbeta, ws, true, T, padding_idx, stream);
 }

@@ -35,6 +35,7 @@ def load() -> ctypes.CDLL:
         _lib.spn_attn_dropbits_elems.restype = ctypes.c_long
         _lib.spn_attn_band_elems.restype = ctypes.c_long
         _lib.spn_gemm_workspace_bytes.restype = ctypes.c_size_t
+        _lib.spn_embed_bwd_det_workspace_floats.restype = ctypes.c_long
         _lib.spn_tuning_name.restype = ctypes.c_char_p
         for name, types in _SIGNATURES.items():
             getattr(_lib, name).argtypes = types
@@ -55,6 +56,7 @@ _SIGNATURES = {
     "spn_paged_append": [_P] * 2 + [_I] + [_L] * 4 + [_P] * 2 + [_I, _P, _L] + [_I] * 3 + [_P],
     "spn_paged_attn": [_P, _L, _L, _P, _P, _I, _P, _L, _P, _P, _P, _L, _L] + [_I] * 6 + [_F, _P, _Z, _P],
     "spn_paged_attn_workspace_bytes": [_I] * 6,
+    "spn_embed_bwd_det_workspace_floats": [_I] * 2,
 }
 
 ABI_VERSION = 10

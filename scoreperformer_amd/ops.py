@@ -603,7 +603,8 @@ def embed_fwd(tables, tokens, gamma, beta, eps: float = 1e-5):
 
 
 def embed_bwd(tables, tokens, dy, gamma, mean, rstd, *, dgamma=None, dbeta=None, padding_idx: int = 0, out=None):
-    """Returns list of dtables (fp32, fresh -- or `out`: contiguous fp32 [V, E] tensors the kernel ADDS to); dgamma/dbeta accumulated in place."""
+    """Returns list of dtables (fp32, fresh -- or `out`: contiguous fp32 [V, E] tensors the kernel ADDS to); dgamma/dbeta accumulated in place, their
+    sums over the rows in a fixed order."""
     tokens, B, t_len, tbs, tts = _tok_view(tokens)
     T = B * t_len
     V = [t.shape[0] for t in tables]
@@ -621,10 +622,11 @@ def embed_bwd(tables, tokens, dy, gamma, mean, rstd, *, dgamma=None, dbeta=None,
         for v, e in zip(V, E):
             dts.append(buf[off:off + v * e].view(v, e))
             off += v * e
-    ws = torch.empty(2 * T, device=dev, dtype=F32) if gamma is not None else None
-    call("spn_embed_bwd", c_int(len(tables)), _ptr_array(tables), _ptr_array(dts), _int_array(V), _int_array(E), ptr(tokens),
+    floats = load().spn_embed_bwd_det_workspace_floats(T, sum(E)) if gamma is not None else 0
+    ws = torch.empty(floats, device=dev, dtype=F32) if floats else None
+    call("spn_embed_bwd_det", c_int(len(tables)), _ptr_array(tables), _ptr_array(dts), _int_array(V), _int_array(E), ptr(tokens),
          c_long(tbs), c_long(tts), c_int(t_len), ptr(dy2), c_long(dy2.stride(0)), ptr(gamma), ptr(mean), ptr(rstd), ptr(dgamma),
-         ptr(dbeta), ptr(ws), c_int(T), c_int(padding_idx), stream_ptr())
+         ptr(dbeta), ptr(ws), c_long(floats), c_int(T), c_int(padding_idx), stream_ptr())
     return dts
 
 
