@@ -23,6 +23,18 @@ class SpnError(RuntimeError):
     pass
 
 
+class SpnMissing(SpnError, AttributeError):
+    """The loaded library was built before this entry point was added."""
+
+
+class _Library(ctypes.CDLL):
+    def __getattr__(self, name):
+        try:
+            return super().__getattr__(name)
+        except AttributeError:
+            raise SpnMissing(f"{LIB_PATH} has no {name}: rebuild it") from None
+
+
 def load() -> ctypes.CDLL:
     """Load libspn.so (built by ``scoreperformer_amd.build``); raises if it is absent."""
     global _lib
@@ -30,18 +42,17 @@ def load() -> ctypes.CDLL:
         if not os.path.exists(LIB_PATH):
             raise SpnError(f"{LIB_PATH} not found: run `python -m scoreperformer_amd.build` "
                            f"(the HIP extension is mandatory; there is no fallback path)")
-        _lib = ctypes.CDLL(LIB_PATH)
-        _lib.spn_last_error.restype = ctypes.c_char_p
-        _lib.spn_attn_dropbits_elems.restype = ctypes.c_long
-        _lib.spn_attn_band_elems.restype = ctypes.c_long
-        _lib.spn_gemm_workspace_bytes.restype = ctypes.c_size_t
-        _lib.spn_embed_bwd_det_workspace_floats.restype = ctypes.c_long
-        _lib.spn_tuning_name.restype = ctypes.c_char_p
+        handle = _Library(LIB_PATH)
+        if handle.spn_abi_version() != ABI_VERSION:
+            raise SpnError(f"{LIB_PATH} has ABI version {handle.spn_abi_version()}, this package needs {ABI_VERSION}: rebuild it")
+        # (a library of the same version built before an entry point was added serves everything else)
+        for name, result in _RESULTS.items():
+            if hasattr(handle, name):
+                getattr(handle, name).restype = result
         for name, types in _SIGNATURES.items():
-            getattr(_lib, name).argtypes = types
-        _lib.spn_paged_attn_workspace_bytes.restype = _lib.spn_paged_plan_workspace_bytes.restype = ctypes.c_size_t
-        if _lib.spn_abi_version() != ABI_VERSION:
-            raise SpnError(f"{LIB_PATH} has ABI version {_lib.spn_abi_version()}, this package needs {ABI_VERSION}: rebuild it")
+            if hasattr(handle, name):
+                getattr(handle, name).argtypes = types
+        _lib = handle
         _apply_env_tuning(_lib)
     return _lib
 
@@ -57,6 +68,13 @@ _SIGNATURES = {
     "spn_paged_attn": [_P, _L, _L, _P, _P, _I, _P, _L, _P, _P, _P, _L, _L] + [_I] * 6 + [_F, _P, _Z, _P],
     "spn_paged_attn_workspace_bytes": [_I] * 6,
     "spn_embed_bwd_det_workspace_floats": [_I] * 2,
+}
+
+# what the entry points return that do not return a status
+_RESULTS = {
+    "spn_last_error": ctypes.c_char_p, "spn_tuning_name": ctypes.c_char_p, "spn_attn_dropbits_elems": c_long, "spn_attn_band_elems": c_long,
+    "spn_gemm_workspace_bytes": _Z, "spn_paged_attn_workspace_bytes": _Z, "spn_paged_plan_workspace_bytes": _Z,
+    "spn_embed_bwd_det_workspace_floats": c_long,
 }
 
 ABI_VERSION = 10
