@@ -1590,9 +1590,11 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
     if slopes is not None and (slopes.dtype is not F32 or slopes.shape != (h,) or not slopes.is_contiguous()):
         raise SpnError(f"{n}: slopes must be contiguous fp32 [{h}]")
     if out is not None:
+        if out.shape != shape:
+            raise SpnError(f"{n}: out must be like q {list(shape)}, got {list(out.shape)}")
         (o_rs, o_hs, inner), d = out.stride(), PAGED_HEAD
         apart = ((h == 1 or o_hs >= d) and (R == 1 or o_rs >= (h - 1) * o_hs + d)) or ((R == 1 or o_rs >= d) and (h == 1 or o_hs >= (R - 1) * o_rs + d))
-        if out.shape != shape or out.dtype is not q.dtype or inner != 1 or not (apart or R == 0):
+        if out.dtype is not q.dtype or inner != 1 or not (apart or R == 0):
             raise SpnError(f"{n}: out must be like q, with unit inner stride and rows that do not overlap")
     dev = _paged_device(n, q, k_pages, v_pages, block_table, lens, slopes, out)
     if out is None:
