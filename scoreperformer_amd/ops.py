@@ -1547,7 +1547,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     n = "paged_append"
     num_pages, kvh, page = _paged_pools(n, k_pages, v_pages)
     _paged_size(n, page)
-    _paged_check(n, k_pages.data_ptr() != v_pages.data_ptr(), "k_pages and v_pages are the same memory")
+    _paged_check(n, abs(k_pages.data_ptr() - v_pages.data_ptr()) >= k_pages.nbytes, "k_pages and v_pages are the same memory")
     T = slots.numel()
     want, ks, vs = (T, kvh, PAGED_HEAD), k.stride(), v.stride()
     if k.shape != want or ks[2] != 1:
