@@ -88,3 +88,44 @@ def attn(q, k_pages, v_pages, table, lens, scale: Optional[float] = None, slopes
             p = torch.softmax(s, 0)
             out[r, hi] = p @ v[hi * kvh // h]
     return out
+
+
+def attn_and_bound(q, k_pages, v_pages, table, lens, scale: Optional[float] = None, slopes=None):
+    """`attn` and, element by element, how far 32-bit arithmetic may be from it (u = 2^-24, w the weights of a request's rows under one head).
+
+    A score: its 64 products sum to A in absolute value; 64 roundings of partial sums that are independent and at most A give 8 u A (their worst case,
+    64 u A, needs every partial sum at A and every rounding to one side); scale, slope and their products are rounded a few times each, the running
+    reference (at most 6 from the largest score) whenever it moves.  The exponential is off by one unit in the last place and by its argument's
+    rounding.  Together a relative error d_j of every weight, which moves the output by at most sum_j w_j d_j (|v_j| + |o|).  Sums over n rows:
+    independent roundings again, 2 sqrt(n) u of the absolute terms, and 16 u for joining waves and parts, in numerator and denominator.
+    bf16 pools: a weight that enters the product as two bf16 terms keeps 2^-16 of itself, and the output is rounded once (2^-8; fp32: u)."""
+    u, bf = 2.0 ** -24, q.dtype == torch.bfloat16
+    R, h, d = q.shape
+    num_pages, kvh, page, _ = k_pages.shape
+    scale = HEAD ** -0.5 if scale is None else scale
+    out, tol = (torch.zeros(R, h, d, dtype=torch.float64) for _ in range(2))
+    for r in range(R):
+        n = min(max(int(lens[r]), 0), table.shape[1] * page)
+        ids = table[r, :pages_of(n, page)].long()
+        there = ((ids >= 0) & (ids < num_pages)).repeat_interleave(page)[:n]
+        j = torch.arange(n)[there]
+        if len(j) == 0:
+            continue
+        rows = ids[j // page] * page + j % page
+        k, v = (p.transpose(1, 2).reshape(-1, kvh, d)[rows].double() for p in (k_pages, v_pages))       # [rows, kvh, d]
+        dist = (n - 1 - j).double()
+        for hi in range(h):
+            kh, vh = k[:, hi * kvh // h], v[:, hi * kvh // h]
+            slope = float(slopes[hi]) if slopes is not None else 0.0
+            products = scale * kh * q[r, hi].double()
+            s, bias = products.sum(1), slope * dist
+            x = s - bias
+            top = x.max()
+            w = torch.softmax(x, 0)
+            o = w @ vh
+            rel = u * (8 * products.abs().sum(1) + 4 * s.abs() + 4 * bias.abs() + 60 * abs(slope) + 6 * (top.abs() + 6) + (x - top).abs() + 4)
+            if bf:
+                rel = rel + 2.0 ** -16
+            out[r, hi] = o
+            tol[r, hi] = (w * rel) @ (vh.abs() + o.abs()) + 2 * (16 + 2 * len(j) ** 0.5) * u * (w @ vh.abs()) + o.abs() * (2.0 ** -8 if bf else u)
+    return out, tol
