@@ -6,8 +6,8 @@
 // maximum, NU independent exponentials and the sums in u order, and the batch joins the running (max, normaliser, weighted values) with
 // one rescale.  The key-by-key online update it replaces (softmax state rescaled after every key: a chain of ~25 dependent instructions
 // per key) took 3 us for 16 keys on the critical path of a note; this form ~0.6 us.
-// Round 5: NU = 8 on EIGHT waves (32 lane groups) instead of 16 on four: a wave issues one instruction per ~5 clocks whatever its
-// neighbour on the SIMD does (tools/pk_probe.hip), the batch is ~45 instructions per key, and the other four waves of the persistent
+// NU = 8 on EIGHT waves (32 lane groups) instead of 16 on four: a wave issues one instruction per ~5 clocks whatever its neighbour on the SIMD
+// does (tools/pk_probe.hip), so its ~45 instructions per key are latency that a second wave halves, and the other four waves of the persistent
 // launch's workgroups had nothing to do during this phase.  Both decode paths use the same NU (the grouping is part of the arithmetic).
 // attention.py:162-197 / attend.py:58-126 semantics: scores q.k * scale - slope * (t - j), softmax over the prefix.
 #pragma once

@@ -4,9 +4,11 @@
 //
 // Every cached row is read once: 2 * kvh * 64 * sizeof(T) bytes per row against 4 * h * 64 flop -- bound by HBM for every head layout, as long
 // as enough loads are in flight, and below some 10 MB by the chain length -> page id -> rows -> softmax -> sum of one workgroup (4 us).
-//  * A segment (request, key head, 16 query heads of it) is one workgroup's, or is cut into parts of at most a 512th of the batch's rows: the
-//    device counts the batch itself, so no length is known to the host and one long cache among short ones does not set the time; a fixed grid
-//    walks the parts, so a table far wider than the lengths costs the second launch and little else.  Parts leave (max, sum, unnormalised o) in the workspace; a second, small launch joins them in a fixed order.
+//  * A segment (request, key head, 16 query heads of it) is one workgroup's, or is cut into parts: of a 512th of the batch's tiles, but at least
+//    MIN_TILES and at most max_tiles of them, and of a 128th of the segment where that is more (a lone request of 131072 rows).  The device counts
+//    the batch itself, so no length is known to the host and one long cache among short ones does not set the time; a fixed grid walks the parts, so
+//    a table far wider than the lengths costs the second launch and the imbalance of the lengths.  Parts leave (max, sum, unnormalised o) in the
+//    workspace; a second, small launch joins them in a fixed order.
 //  * Rows travel HBM -> LDS by DMA in whole 1 KiB pieces, 16 bytes a lane, consecutive lanes on consecutive bytes.  (The layouts the matrix
 //    instructions want, loaded straight into registers -- a lane per row, 64 of a row's 128 bytes at a time -- hold one CU to 37 GB/s where
 //    whole pieces reach 105: the first-level cache serves four lanes of one line per clock.)  Two tiles of 8 KiB per wave, private to it: no barrier.
@@ -14,8 +16,9 @@
 //    K is read from LDS by rows, V by transposing reads (bf16) or one row element per lane (fp32), both without bank conflicts.
 //  * The query heads of one key head are the 16 columns of the tile; fewer leave columns idle, which costs nothing; more are further segments.
 //  * fp32 pools: v_mfma_f32_16x16x4_f32, products and sums in fp32.  bf16 pools: products exact, sums in fp32, and a probability enters the
-//    second product as TWO bf16 terms (its rounding and the remainder): 2^-17 instead of 2^-9 of it, for 5 more matrix instructions per tile in
-//    a kernel that waits for memory -- the output then carries one bf16 rounding, not two.
+//    second product as TWO bf16 terms (its rounding and the remainder): off by at most 2^-16 of it instead of 2^-8, for 5 more matrix instructions
+//    per tile in a kernel that waits for memory -- the output then carries one bf16 rounding, not two.  fp32 errors are 1.3 - 1.5 times those of a
+//    softmax in elementary fp32 operations (2.1e-7 against 1.5e-7 of the output, 32 x 1 .. 4096).
 //  * A wave instruction takes its SIMD four clocks, so what is the same for a whole tile or walk is kept off the vector unit: page ids, their
 //    checks and the addresses are scalar; the bias inside a tile is the C operand of the score product; the running maximum is compared lane by
 //    lane and reduced over lanes only when it moves by more than RISE; the sum of the probabilities is one more row of the value product.
@@ -42,12 +45,13 @@ struct PagedAttnArgs {
     void* o; long o_rs, o_hs; int R, h, kvh, W, num_pages, shift; float scale;
     int group, passes;         // query heads per key head, 16-head passes over them
     int rows;                  // heads of a partial result: min(group, 16)
-    int max_tiles;             // most tiles of a part
+    int max_tiles;             // longest part aimed at, in tiles (more where a segment would have more than MAX_PARTS of them)
     int once;                  // whole segments: do not keep the rows in the caches (cut ones: decided on the device)
     int units;                 // room for this many parts
     float* part; float* ml;    // [units][rows][64], [units][rows][2]
-    int4* hdr;                 // {parts of the batch, most tiles of one, once, 0}, [units] {request, key head and pass, parts (its first part only), 0}
-    int* line;                 // batches of more than SEARCH requests: [R] parts of the requests before this one}
+    int4* hdr;                 // {parts of the batch; behind paged_line_kernel also: longest part aimed at, once, parts are short; otherwise 0},
+                               // [units] {request, key head and pass, parts (its first part only), 0}
+    int* line;                 // batches of more than SEARCH requests: [R] parts of the requests before this one
 };
 
 // reductions over the four lanes of a head (l, l ^ 16, l ^ 32, l ^ 48): the swapped halves of two copies, no LDS crossbar
@@ -485,7 +489,7 @@ __global__ __launch_bounds__(LINE_T) void paged_line_kernel(PagedAttnArgs a) {
     if (tid == 0) a.hdr[0] = int4{min(carry, a.units), most, total * STAGE >= ONCE, total <= (long)carry * (SHORT / 2)};
 }
 
-// Segments cut into parts: a TARGET-th of the batch's tiles is the longest part, the parts of all segments stand in one line, of which workgroup g takes
+// Segments cut into parts (paged_split.h most_of, parts_of): the parts of all segments stand in one line, of which workgroup g takes
 // number g, g + G, ...  (four at a time where there are enough of them, and short).  SEARCHED: the line was drawn by the kernel above; otherwise
 // every wave draws it for itself (a lane: every 64th stretch of requests; no barrier, no LDS, no launch).
 template <typename T, bool SEARCHED>

@@ -10,7 +10,7 @@ constexpr int HEADS = 16;           // query heads of a segment
 constexpr int STAGE = 8192;         // bytes of a tile: 4 KiB of keys, 4 KiB of values
 constexpr int MIN_TILES = 4;        // least tiles of a part (a tile per wave; 2: the same, 8: 1 x 4096 rows 8.9 -> 8.2 us the other way)
 constexpr int TARGET = 512;         // parts the batch is cut into, beside one per segment (1024: the same within 2 %)
-constexpr int MAX_TILES = 64;       // most tiles of a part where the batch is larger (32: 256 x 4096 rows 182 -> 196 us, 128: 186)
+constexpr int MAX_TILES = 64;       // longest part aimed at where the batch is larger (32: 256 x 4096 rows 182 -> 196 us, 128: 186)
 constexpr int RESIDENT = 512;       // workgroups of 4 waves that run at once: two on a compute unit, by their LDS
 constexpr unsigned GRID = 2 * RESIDENT;   // workgroups of a cut batch
 constexpr int MAX_PARTS = 128;      // parts of a segment (one of 131072 rows, 256: 18.9 us, 128: 17.2, 64: 20.8 when a tile cost a tenth more)
@@ -30,7 +30,7 @@ SPN_HD int parts_of(int tiles, int most) {
     return parts < 1 ? 1 : parts < MAX_PARTS ? parts : MAX_PARTS;
 }
 
-// the longest part of a batch of `total` tiles
+// the longest part aimed at in a batch of `total` tiles
 SPN_HD int most_of(long total, int max_tiles) {
     const long even = (total + TARGET - 1) / TARGET, most = even < MIN_TILES ? MIN_TILES : even;
     return (int)(most < max_tiles ? most : max_tiles);

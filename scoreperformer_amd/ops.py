@@ -1572,7 +1572,8 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bl
 
     q [R, h, 64] (any strides with unit inner stride) and the pages [num_pages, kv_heads, page, 64] both bf16 or both fp32; kv_heads divides h (1:
     multi-query); block_table [R, W] and lens [R] int32; slopes [h] fp32 (ALiBi) or None; scale defaults to 1 / 8.  Returns [R, h, 64] in q's dtype
-    (`out` if given: `q` itself, or memory of its own).  Scores, softmax and sums in fp32.  A request of length 0 has zeros, and so has a head whose
+    (`out` if given: `q` itself, or memory of its own).  Scores, softmax and sums in fp32, the sums relative to a weight of up to 2^8: values beyond
+    2^119 / cached rows can pass its range.  A request of length 0 has zeros, and so has a head whose
     visible scores are all -infinity; an infinite or NaN value in a visible row makes its dimension NaN or infinite.  Rows on an entry outside
     [0, num_pages) are skipped as if masked (positions count on), rows behind a length are never read into a result, and a length past the
     table's W pages is cut to them.
