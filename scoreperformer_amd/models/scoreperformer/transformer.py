@@ -107,7 +107,7 @@ class TupleTransformer(nn.Module, Constructor):
         given = [("x", x)] + [("x_extra", t) for t in extra if hasattr(self.token_emb, "multiseq_mode")]
         if self.context_emb_mode == EmbeddingModes.CONCAT:
             given.append(("context", context))
-        if style is not None and (self.style_emb_mode == EmbeddingModes.CONCAT or style.shape[1] != 1):
+        if style is not None and (self.style_emb_mode == EmbeddingModes.CONCAT or (self.transformer.ada_norm and style.shape[1] != 1)):
             given.append(("style_embeddings", style))
         for name, t in given:
             if t is not None and t.shape[:2] != step.slots.shape:

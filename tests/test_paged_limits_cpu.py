@@ -97,6 +97,34 @@ def test_tiles_of_any_length(tmp_path):
     _host_check(tmp_path, TILES)
 
 
+INDEX = HEAD + r"""
+int main() {
+    const int R = 1, h = 1, kvh = 1, esize = 2;
+    for (int it = 0; it < 2000000; ++it) {
+        const int shift = 3 + std::rand() % 10, W = it % 3 ? lg(2147483647.0) : INT_MAX - std::rand() % 100;
+        const int len = it % 5 ? lg(2147483647.0) : INT_MAX - std::rand() % 5000, fresh = lg(2147483647.0), width = INT_MAX;
+        // a release walks the held pages 64 at a time: the walk's end stays an int for any width of the table
+        const long held = pages_of(len, shift) < W ? pages_of(len, shift) : W;
+        NEED(held >= 0 && held <= (1 << 28) && held + 64 <= INT_MAX);
+        const int need = pages_needed(len, fresh, width, W, shift);
+        NEED(need >= -1 && (need < 0 || pages_of(len, shift) + need <= W));
+        NEED(need < 0 || pages_of((long)len + fresh, shift) == pages_of(len, shift) + need);
+        if (((long)W << shift) >= (1L << 31)) continue;                                     // (refused by plan and attention)
+        const int n = rows_of(len, W, shift);
+        NEED(n <= len && n <= (long)W << shift && (n == 0 || ((n - 1) >> shift) < W));
+        NEED(need < 0 || (long)len + fresh <= INT_MAX);                                     // the new length is an int
+    }
+    std::puts("ok");
+    return 0;
+}
+"""
+
+
+def test_index_arithmetic_at_the_widest_tables(tmp_path):
+    """Tables of up to 2^31 - 1 entries a row: plan's counts, release's walk, the rows that the attention takes."""
+    _host_check(tmp_path, INDEX)
+
+
 QUERY = """
 import ctypes, sys
 lib = ctypes.CDLL(sys.argv[1])
